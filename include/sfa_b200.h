@@ -294,6 +294,63 @@ typedef struct SfaIndexerParams {
 size_t sfa_indexer_workspace_bytes(const SfaIndexerParams* p);
 int sfa_indexer_topk(const SfaIndexerParams* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Norm and rotary positions of queries and keys: the step before the op (no
+ * counterpart in the reference, which takes q and kv as they are, SFA.py:87-90).
+ * For every row x (one head of one token, dim elements), in fp32:
+ *     n = x * rsqrt(mean(x^2) + eps) * weight          (tensors with a weight)
+ *     y = n with the pairs of its dims [start, start + rot) turned by
+ *         position * frequencies[i] and scaled by amplitude (SFA_ROTARY_TURN)
+ * rounded once to the tensor's type.  Pair i is (i, i + rot/2) of the rotated
+ * part, or (2i, 2i + 1) when interleaved.  Angles are reduced exactly: the
+ * position multiplies the frequency as a 64-bit fraction of a turn, so far
+ * positions keep full accuracy.
+ *
+ * Up to three tensors go through one launch (q, k and, for the append, v with
+ * neither weight nor TURN).  A tensor with SFA_ROTARY_PAGED is stored into a
+ * page pool instead: y is the pool, y_st its row stride, y_sh its head stride;
+ * batch must be 1 and row i of sequence s (cu_seqlens; NULL: one row each) goes
+ * to cache position cache_seqlens[s] - rows(s) + i through block_table.  Rows
+ * behind cu_seqlens[num_seqs], negative positions, positions behind the table
+ * and page ids outside [0, num_pages) are not stored.
+ * Backward: dx from x and dy, dweight (fp32, overwritten, fixed summation order). */
+enum { SFA_DTYPE_BF16 = 0, SFA_DTYPE_F16 = 1, SFA_DTYPE_F32 = 2 };
+enum { SFA_ROTARY_TURN = 1, SFA_ROTARY_PAGED = 2 };
+
+typedef struct SfaRotaryTensor {
+  const void* x;
+  void* y;               /* forward output (or the page pool) */
+  const void* dy;        /* backward */
+  void* dx;
+  const float* weight;   /* [dim] or NULL: no norm */
+  float* dweight;        /* [dim] or NULL */
+  int64_t x_sb, x_st, x_sh;   /* element strides: batch, token, head */
+  int64_t y_sb, y_st, y_sh;
+  int64_t dy_sb, dy_st, dy_sh;
+  int64_t dx_sb, dx_st, dx_sh;
+  int32_t heads;
+  int32_t flags;         /* SFA_ROTARY_* */
+} SfaRotaryTensor;
+
+typedef struct SfaRotaryParams {
+  SfaRotaryTensor t[3];
+  const void* positions;        /* int32, or int64 with pos64 */
+  const double* frequencies;    /* [rot / 2] radians per position */
+  const int32_t* block_table;   /* paged tensors only, from here ... */
+  const int32_t* cache_seqlens;
+  const int32_t* cu_seqlens;
+  int64_t bt_stride;            /* ... to here */
+  int64_t p_sb, p_st;
+  int32_t num_tensors, batch, len, dim, rot, start, interleaved, dtype, pos64;
+  int32_t num_seqs, num_pages, page_size, table_width;
+  float eps, amplitude;
+  int32_t reserved;
+} SfaRotaryParams;
+
+int sfa_rotary_fwd(const SfaRotaryParams* p, void* stream);
+size_t sfa_rotary_bwd_workspace_bytes(const SfaRotaryParams* p);
+int sfa_rotary_bwd(const SfaRotaryParams* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

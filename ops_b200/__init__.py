@@ -6,6 +6,9 @@ Public surface:
   sparse_flash_attention_paged(q, k_cache, v_cache, block_indices, block_table, cache_seqlens, ...)
                                                       # forward over a paged kv cache (decode)
   lightning_indexer_topk(q_idx, k_idx, weights, topk) -> token indices for the op
+  rotary_frequencies / rotary_embedding / qk_norm_rotary(q, k, positions, frequencies, ...)
+                                                      # norm and rotary positions before the op, with gradients
+  qk_norm_rotary_append(q, k, v, ..., k_cache, v_cache, block_table, cache_seqlens)   # the same into a paged cache
   sparse_flash_attention_fp8kv(q, kv_fp8, kv_scale, block_indices, d_v, ...)  # e4m3 latent kv cache
 The kernels live in libsfa_b200.so (C ABI: include/sfa_b200.h).
 """
@@ -14,7 +17,9 @@ from .sfa import (SparseFlashAttention, SparseFlashAttentionCompat, quantize_kv_
                   sparse_flash_attention, sparse_flash_attention_fp8kv, sparse_flash_attention_paged)
 from . import tiling
 from .indexer import lightning_indexer_topk
+from .rotary import qk_norm_rotary, qk_norm_rotary_append, rotary_embedding, rotary_frequencies
 
 __all__ = ["sparse_flash_attention", "sparse_flash_attention_paged", "SparseFlashAttention",
            "SparseFlashAttentionCompat", "SfaError", "SfaParams", "load_library", "reference_lse2", "tiling",
-           "lightning_indexer_topk", "sparse_flash_attention_fp8kv", "quantize_kv_fp8"]
+           "lightning_indexer_topk", "sparse_flash_attention_fp8kv", "quantize_kv_fp8", "rotary_frequencies",
+           "rotary_embedding", "qk_norm_rotary", "qk_norm_rotary_append"]

@@ -24,6 +24,8 @@ SFA_KERNEL_AUTO, SFA_KERNEL_TCGEN05, SFA_KERNEL_GENERAL = 0, 1, 2
 SFA_DQ_AUTO, SFA_DQ_SEPARATE, SFA_DQ_FUSED = 0, 1, 2
 SFA_COMPAT_REFERENCE_P = 1
 SFA_KV_BF16, SFA_KV_FP8_E4M3 = 0, 1
+SFA_DTYPE_BF16, SFA_DTYPE_F16, SFA_DTYPE_F32 = 0, 1, 2
+SFA_ROTARY_TURN, SFA_ROTARY_PAGED = 1, 2
 SFA_SELFTEST_STATUS = (15 << 16) | 1   # status code of sfa_selftest_wait_timeout
 
 _c_void_p = ctypes.c_void_p
@@ -64,6 +66,26 @@ class SfaIndexerParams(ctypes.Structure):
     ]
 
 
+class SfaRotaryTensor(ctypes.Structure):
+    """Field-for-field mirror of ``SfaRotaryTensor`` in include/sfa_b200.h."""
+
+    _fields_ = [("x", _c_void_p), ("y", _c_void_p), ("dy", _c_void_p), ("dx", _c_void_p), ("weight", _c_void_p),
+                ("dweight", _c_void_p)
+                ] + [(f"{t}_{s}", _i64) for t in ("x", "y", "dy", "dx") for s in ("sb", "st", "sh")] + [
+        ("heads", _i32), ("flags", _i32)]
+
+
+class SfaRotaryParams(ctypes.Structure):
+    """Field-for-field mirror of ``SfaRotaryParams`` in include/sfa_b200.h."""
+
+    _fields_ = [
+        ("t", SfaRotaryTensor * 3), ("positions", _c_void_p), ("frequencies", _c_void_p), ("block_table", _c_void_p),
+        ("cache_seqlens", _c_void_p), ("cu_seqlens", _c_void_p), ("bt_stride", _i64), ("p_sb", _i64), ("p_st", _i64),
+    ] + [(n, _i32) for n in ("num_tensors", "batch", "len", "dim", "rot", "start", "interleaved", "dtype", "pos64",
+                             "num_seqs", "num_pages", "page_size", "table_width")] + [
+        ("eps", ctypes.c_float), ("amplitude", ctypes.c_float), ("reserved", _i32)]
+
+
 EXPORTS = {
     "sfa_abi_version": ([], _i32),
     "sfa_build_info": ([], ctypes.c_char_p),
@@ -90,6 +112,9 @@ EXPORTS = {
     "sfa_launch_trace_count": ([], _i32),
     "sfa_launch_trace_name": ([_i32], ctypes.c_char_p),
     "sfa_indexer_workspace_bytes": ([ctypes.POINTER(SfaIndexerParams)], ctypes.c_size_t),
+    "sfa_rotary_fwd": ([ctypes.POINTER(SfaRotaryParams), _c_void_p], _i32),
+    "sfa_rotary_bwd_workspace_bytes": ([ctypes.POINTER(SfaRotaryParams)], ctypes.c_size_t),
+    "sfa_rotary_bwd": ([ctypes.POINTER(SfaRotaryParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_indexer_topk": ([ctypes.POINTER(SfaIndexerParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
 }
 
