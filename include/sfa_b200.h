@@ -351,6 +351,56 @@ int sfa_rotary_fwd(const SfaRotaryParams* p, void* stream);
 size_t sfa_rotary_bwd_workspace_bytes(const SfaRotaryParams* p);
 int sfa_rotary_bwd(const SfaRotaryParams* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Attention of drafted tokens over a paged kv cache (no counterpart in the
+ * reference): every query row sees all of its sequence's cache rows before the
+ * drafted ones, and of the drafted ones its own and its ancestors'.
+ *
+ * q [total_q, h_q, d_qk] holds the drafted rows of num_seqs sequences, offsets
+ * cu_seqlens (NULL: one row each); cache_seqlens are the cache lengths with
+ * them, so row j of sequence s is cache position cache_seqlens[s] - rows(s) + j.
+ * parents[row] is the row's parent within its sequence (a number below its own;
+ * anything else: the row hangs on the prefix); NULL: a chain (causal).  With
+ * parents a sequence has at most SFA_TREE_MAX_NODES rows.  Keys and values are
+ * read through block_table from pools of num_pages pages; a table entry outside
+ * [0, num_pages) and positions behind the table hold no keys.  Values of cache
+ * rows that no row of the sequence sees do not matter, NaN included, and a row
+ * is not touched by what a drafted row it does not see holds.  attn_sink adds
+ * exp(sink) to the denominator.  A row that sees nothing gives o = 0 and lse =
+ * -inf (or its sink); so do rows behind cu_seqlens[num_seqs].
+ * Types: bf16 or fp16 (dtype), lse fp32; d_qk and d_v multiples of 8 up to 256;
+ * strides in elements, multiples of 8, bases 16-byte aligned; scale > 0. */
+#define SFA_TREE_MAX_NODES 256
+
+typedef struct SfaTreeParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* block_table;
+  const int32_t* cache_seqlens;
+  const int32_t* cu_seqlens;
+  const int32_t* parents;
+  const float* attn_sink;
+  void* o;
+  float* lse;
+  int64_t q_st, q_sh;
+  int64_t k_st, k_sh;   /* pool row and head strides; page p is rows [p*page_size, (p+1)*page_size) */
+  int64_t v_st, v_sh;
+  int64_t o_st, o_sh;
+  int64_t l_st, l_sh;
+  int64_t bt_stride;
+  int32_t num_seqs, total_q;
+  int32_t max_q;        /* the most rows of a sequence */
+  int32_t max_k;        /* an estimate of the longest cache (sizes the split; not a limit) */
+  int32_t h_q, h_kv, d_qk, d_v;
+  int32_t num_pages, page_size, table_width, dtype;
+  float scale;
+  int32_t reserved;
+} SfaTreeParams;
+
+size_t sfa_tree_workspace_bytes(const SfaTreeParams* p);
+int sfa_tree_attention(const SfaTreeParams* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

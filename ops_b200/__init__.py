@@ -6,6 +6,8 @@ Public surface:
   sparse_flash_attention_paged(q, k_cache, v_cache, block_indices, block_table, cache_seqlens, ...)
                                                       # forward over a paged kv cache (decode)
   lightning_indexer_topk(q_idx, k_idx, weights, topk) -> token indices for the op
+  tree_attention_paged(q, k_cache, v_cache, block_table, cache_seqlens, parents, ...)
+                                                      # drafted trees, chains or single tokens over the whole cache
   rotary_frequencies / rotary_embedding / qk_norm_rotary(q, k, positions, frequencies, ...)
                                                       # norm and rotary positions before the op, with gradients
   qk_norm_rotary_append(q, k, v, ..., k_cache, v_cache, block_table, cache_seqlens)   # the same into a paged cache
@@ -17,9 +19,10 @@ from .sfa import (SparseFlashAttention, SparseFlashAttentionCompat, quantize_kv_
                   sparse_flash_attention, sparse_flash_attention_fp8kv, sparse_flash_attention_paged)
 from . import tiling
 from .indexer import lightning_indexer_topk
+from .tree import tree_attention_paged
 from .rotary import qk_norm_rotary, qk_norm_rotary_append, rotary_embedding, rotary_frequencies
 
 __all__ = ["sparse_flash_attention", "sparse_flash_attention_paged", "SparseFlashAttention",
            "SparseFlashAttentionCompat", "SfaError", "SfaParams", "load_library", "reference_lse2", "tiling",
            "lightning_indexer_topk", "sparse_flash_attention_fp8kv", "quantize_kv_fp8", "rotary_frequencies",
-           "rotary_embedding", "qk_norm_rotary", "qk_norm_rotary_append"]
+           "rotary_embedding", "tree_attention_paged", "qk_norm_rotary", "qk_norm_rotary_append"]

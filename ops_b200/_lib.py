@@ -26,6 +26,7 @@ SFA_COMPAT_REFERENCE_P = 1
 SFA_KV_BF16, SFA_KV_FP8_E4M3 = 0, 1
 SFA_DTYPE_BF16, SFA_DTYPE_F16, SFA_DTYPE_F32 = 0, 1, 2
 SFA_ROTARY_TURN, SFA_ROTARY_PAGED = 1, 2
+SFA_TREE_MAX_NODES = 256
 SFA_SELFTEST_STATUS = (15 << 16) | 1   # status code of sfa_selftest_wait_timeout
 
 _c_void_p = ctypes.c_void_p
@@ -86,6 +87,16 @@ class SfaRotaryParams(ctypes.Structure):
         ("eps", ctypes.c_float), ("amplitude", ctypes.c_float), ("reserved", _i32)]
 
 
+class SfaTreeParams(ctypes.Structure):
+    """Field-for-field mirror of ``SfaTreeParams`` in include/sfa_b200.h."""
+
+    _fields_ = [(n, _c_void_p) for n in ("q", "k", "v", "block_table", "cache_seqlens", "cu_seqlens", "parents",
+                                         "attn_sink", "o", "lse")] + [
+        (f"{t}_{s}", _i64) for t in ("q", "k", "v", "o", "l") for s in ("st", "sh")] + [("bt_stride", _i64)] + [
+        (n, _i32) for n in ("num_seqs", "total_q", "max_q", "max_k", "h_q", "h_kv", "d_qk", "d_v", "num_pages",
+                            "page_size", "table_width", "dtype")] + [("scale", ctypes.c_float), ("reserved", _i32)]
+
+
 EXPORTS = {
     "sfa_abi_version": ([], _i32),
     "sfa_build_info": ([], ctypes.c_char_p),
@@ -115,6 +126,8 @@ EXPORTS = {
     "sfa_rotary_fwd": ([ctypes.POINTER(SfaRotaryParams), _c_void_p], _i32),
     "sfa_rotary_bwd_workspace_bytes": ([ctypes.POINTER(SfaRotaryParams)], ctypes.c_size_t),
     "sfa_rotary_bwd": ([ctypes.POINTER(SfaRotaryParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
+    "sfa_tree_workspace_bytes": ([ctypes.POINTER(SfaTreeParams)], ctypes.c_size_t),
+    "sfa_tree_attention": ([ctypes.POINTER(SfaTreeParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_indexer_topk": ([ctypes.POINTER(SfaIndexerParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
 }
 

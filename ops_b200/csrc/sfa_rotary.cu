@@ -555,7 +555,8 @@ static int check(const SfaRotaryParams* p, bool bwd) {
   for (int i = 0; i < p->num_tensors; ++i) {
     const SfaRotaryTensor& t = p->t[i];
     if (t.heads < 1) return bad("heads must be positive");
-    if (!empty && (!t.x || (bwd ? !t.dy || !t.dx : !t.y))) return bad("tensor pointers must be non-NULL");
+    const bool no_pool = (t.flags & SFA_ROTARY_PAGED) && p->num_pages == 0;
+    if (!empty && (!t.x || (bwd ? !t.dy || !t.dx : !t.y && !no_pool))) return bad("tensor pointers must be non-NULL");
     if (!empty && (t.flags & SFA_ROTARY_TURN) && p->rot && (!p->positions || !p->frequencies))
       return bad("positions and frequencies must be non-NULL");
     if (bwd && t.dweight && !t.weight) return bad("dweight needs a weight");
@@ -564,7 +565,7 @@ static int check(const SfaRotaryParams* p, bool bwd) {
       if (p->batch != 1 && !empty) return bad("a paged tensor needs batch 1");
       if (p->page_size < 1 || p->num_pages < 0 || p->table_width < 0 || p->num_seqs < 0)
         return bad("page_size must be positive and num_pages, table_width, num_seqs >= 0");
-      if (!empty && p->num_seqs > 0 && (!p->block_table || !p->cache_seqlens))
+      if (!empty && p->num_seqs > 0 && ((p->table_width > 0 && !p->block_table) || !p->cache_seqlens))
         return bad("a paged tensor needs block_table and cache_seqlens");
     }
   }
