@@ -401,6 +401,63 @@ typedef struct SfaTreeParams {
 size_t sfa_tree_workspace_bytes(const SfaTreeParams* p);
 int sfa_tree_attention(const SfaTreeParams* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Pages of a kv cache (no counterpart in the reference).  A pool has num_pages
+ * pages; refcounts[page] says how many block-table entries hold it (0: free).
+ * Sequence s holds its first ceil(cache_seqlens[s] / page_size) table entries;
+ * the entries behind are -1.  New pages are the free ones of lowest number, in
+ * the order of the rows that ask, so results repeat.  All state is on the
+ * device and nothing is read back.  pools (a host array) are the tensors that
+ * the pages index, e.g. K and V of every layer: page p is page_bytes contiguous
+ * bytes at base + p * page_stride.
+ *
+ *  - reserve: a = [num_seqs] rows to add.  out[s] = 1 if s got the pages for
+ *    them (cache_seqlens grows), 0 if nothing was changed: a negative count, a
+ *    table too narrow, a partly filled last page that others share, or free
+ *    pages too few for the rows up to s together;
+ *  - trim: a = [num_seqs] rows to keep (negative: leave s alone).  Entries
+ *    behind them are given back;
+ *  - fork: a = [count] source, b = [count] target sequences.  Whole pages are
+ *    shared, a partly filled last page is copied to a new one.  out[i] = 1 if
+ *    done, 0 if nothing was changed: a number outside the table, a target that
+ *    holds rows or is named by an earlier fork, a last page outside the pool,
+ *    or free pages too few.  Sources are taken as they were before the call;
+ *  - accept: a = [num_seqs, count] accepted drafted rows of each sequence,
+ *    ascending, ended by -1 or the width; b = [num_seqs] drafted rows.  The
+ *    accepted cache rows are moved together behind the prefix, cache_seqlens -
+ *    b; out[s] = rows to keep (for trim), -1 for a sequence with b outside
+ *    [0, cache_seqlens];
+ *  - compact: pages in use are moved to the lowest numbers, refcounts and table
+ *    follow; out[0] = pages in use;
+ *  - copy: page a[i] to page b[i], i < count.  out[i] = 1 if copied, 0 for a
+ *    page outside the pool, a target named by an earlier pair, or a source that
+ *    another pair writes. */
+typedef struct SfaCachePool {
+  void* base;
+  int64_t page_stride;   /* bytes */
+  int64_t page_bytes;    /* a multiple of page_size */
+} SfaCachePool;
+
+typedef struct SfaCacheParams {
+  int32_t* refcounts;
+  int32_t* block_table;
+  int32_t* cache_seqlens;
+  const int32_t* a;
+  const int32_t* b;
+  int32_t* out;
+  const SfaCachePool* pools;   /* host */
+  int64_t bt_stride, a_stride;
+  int32_t num_pools, num_seqs, num_pages, page_size, table_width, count;
+} SfaCacheParams;
+
+size_t sfa_cache_workspace_bytes(const SfaCacheParams* p);   /* enough for every call below */
+int sfa_cache_reserve(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
+int sfa_cache_trim(const SfaCacheParams* p, void* stream);
+int sfa_cache_fork(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
+int sfa_cache_accept(const SfaCacheParams* p, void* stream);
+int sfa_cache_compact(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
+int sfa_cache_copy(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -97,6 +97,20 @@ class SfaTreeParams(ctypes.Structure):
                             "page_size", "table_width", "dtype")] + [("scale", ctypes.c_float), ("reserved", _i32)]
 
 
+class SfaCachePool(ctypes.Structure):
+    """Field-for-field mirror of ``SfaCachePool`` in include/sfa_b200.h."""
+
+    _fields_ = [("base", _c_void_p), ("page_stride", _i64), ("page_bytes", _i64)]
+
+
+class SfaCacheParams(ctypes.Structure):
+    """Field-for-field mirror of ``SfaCacheParams`` in include/sfa_b200.h."""
+
+    _fields_ = [(n, _c_void_p) for n in ("refcounts", "block_table", "cache_seqlens", "a", "b", "out")] + [
+        ("pools", ctypes.POINTER(SfaCachePool)), ("bt_stride", _i64), ("a_stride", _i64)] + [
+        (n, _i32) for n in ("num_pools", "num_seqs", "num_pages", "page_size", "table_width", "count")]
+
+
 EXPORTS = {
     "sfa_abi_version": ([], _i32),
     "sfa_build_info": ([], ctypes.c_char_p),
@@ -128,6 +142,13 @@ EXPORTS = {
     "sfa_rotary_bwd": ([ctypes.POINTER(SfaRotaryParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_tree_workspace_bytes": ([ctypes.POINTER(SfaTreeParams)], ctypes.c_size_t),
     "sfa_tree_attention": ([ctypes.POINTER(SfaTreeParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
+    "sfa_cache_workspace_bytes": ([ctypes.POINTER(SfaCacheParams)], ctypes.c_size_t),
+    "sfa_cache_reserve": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
+    "sfa_cache_trim": ([ctypes.POINTER(SfaCacheParams), _c_void_p], _i32),
+    "sfa_cache_fork": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
+    "sfa_cache_accept": ([ctypes.POINTER(SfaCacheParams), _c_void_p], _i32),
+    "sfa_cache_compact": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
+    "sfa_cache_copy": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_indexer_topk": ([ctypes.POINTER(SfaIndexerParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
 }
 
