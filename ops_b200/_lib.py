@@ -8,6 +8,9 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
+
+import torch
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libsfa_b200.so")
@@ -151,6 +154,60 @@ EXPORTS = {
     "sfa_cache_copy": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_indexer_topk": ([ctypes.POINTER(SfaIndexerParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
 }
+
+_FORMAT = {_c_void_p: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}
+
+
+def _formats(cls) -> str:
+    out = ""
+    for _, t in cls._fields_:
+        if issubclass(t, ctypes.Array):
+            out += _formats(t._type_) * t._length_
+        elif issubclass(t, ctypes.Structure):
+            out += _formats(t)
+        else:
+            out += _FORMAT.get(t, "P")
+    return out
+
+
+def packer(cls):
+    """``f(*values) -> cls`` with every field's value in order (nested ones in
+    place, 0 for a null pointer): one call instead of an attribute write per
+    field, which costs more than a small kernel runs."""
+    pack = struct.Struct("@" + _formats(cls) + "0q").pack
+    make = cls.from_buffer_copy
+    assert struct.calcsize("@" + _formats(cls) + "0q") == ctypes.sizeof(cls)
+
+    def build(*values):
+        return make(pack(*values))
+
+    return build
+
+
+def stream_of(device: torch.device) -> int:
+    """Handle of the device's current stream."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class on:
+    """``with on(device)``: the device is current inside.  Costs one query when it
+    already is, as in almost every call."""
+
+    __slots__ = ("to", "back")
+
+    def __init__(self, device: torch.device):
+        self.to = device.index
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.to:
+            torch.cuda.set_device(self.to)
+
+    def __exit__(self, *exc):
+        if self.back != self.to:
+            torch.cuda.set_device(self.back)
+        return False
+
 
 _lib = None
 

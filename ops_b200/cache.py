@@ -15,13 +15,14 @@ page_size, ...]`` with contiguous pages: K and V of every layer, any type.
 from __future__ import annotations
 
 import ctypes
+import math
+import struct
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
 from ._lib import SfaCacheParams, SfaCachePool
-from .rotary import _stream
 
 
 def _ints(name: str, t: torch.Tensor, dim: int, like: torch.Tensor, size: Optional[int] = None) -> None:
@@ -38,36 +39,40 @@ def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Op
     if len(pools) == 0:
         raise ValueError("pools must hold at least one tensor")
     first = pools[0]
-    arr = (SfaCachePool * len(pools))()
-    for i, t in enumerate(pools):
+    values = []
+    for t in pools:
         if t.dim() < 2 or t.device != like.device or t.shape[1] < 1 or t.shape[:2] != first.shape[:2] or (
                 num_pages is not None and t.shape[0] != num_pages):
             raise ValueError("every pool must be [num_pages, page_size, ...] with the same pages, on the device of the table")
-        inner = t.stride(0) if t.shape[0] > 1 else 0
-        expect = 1
-        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if size > 1 and stride != expect:
-                raise ValueError("a pool's pages must be contiguous")
-            expect *= size
-        if t.shape[0] > 1 and inner < expect:
-            raise ValueError("a pool's pages must not overlap")
+        if t.is_contiguous():
+            inner = expect = math.prod(t.shape[1:])
+        else:
+            inner = t.stride(0) if t.shape[0] > 1 else 0
+            expect = 1
+            for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+                if size > 1 and stride != expect:
+                    raise ValueError("a pool's pages must be contiguous")
+                expect *= size
+            if t.shape[0] > 1 and inner < expect:
+                raise ValueError("a pool's pages must not overlap")
         size = t.element_size()
-        arr[i].base, arr[i].page_stride, arr[i].page_bytes = t.data_ptr(), (inner or expect) * size, expect * size
+        values += (t.data_ptr(), (inner or expect) * size, expect * size)
+    arr = (SfaCachePool * len(pools)).from_buffer_copy(struct.pack("@" + "Pqq" * len(pools), *values))
     return arr, first.shape[0], first.shape[1]
+
+
+_pack = _lib.packer(SfaCacheParams)
 
 
 def _params(refcounts, table, lens, page_size, num_pages, a=None, b=None, out=None, pools=None, count=0) -> SfaCacheParams:
     def ptr(t):
-        return None if t is None else t.data_ptr()
+        return 0 if t is None else t.data_ptr()
 
-    P = SfaCacheParams(refcounts=ptr(refcounts), block_table=ptr(table), cache_seqlens=ptr(lens), a=ptr(a), b=ptr(b),
-                       out=ptr(out), page_size=int(page_size), num_pages=num_pages, count=count)
-    if table is not None:
-        P.num_seqs, P.table_width, P.bt_stride = table.shape[0], table.shape[1], table.stride(0)
-    if a is not None and a.dim() == 2:
-        P.a_stride = a.stride(0)
-    if pools is not None:
-        P.pools, P.num_pools = pools, len(pools)
+    n, width, bt = (0, 0, 0) if table is None else (*table.shape, table.stride(0))
+    a_stride = a.stride(0) if a is not None and a.dim() == 2 else 0
+    P = _pack(ptr(refcounts), ptr(table), ptr(lens), ptr(a), ptr(b), ptr(out), 0 if pools is None else ctypes.addressof(pools),
+              bt, a_stride, 0 if pools is None else len(pools), n, num_pages, int(page_size), width, count)
+    P.held = pools                       # the array lives as long as the struct
     return P
 
 
@@ -75,13 +80,13 @@ def _call(name: str, P: SfaCacheParams, like: torch.Tensor, workspace: bool = Tr
     if not like.is_cuda:
         raise ValueError("the cache's state must be CUDA tensors (there is no CPU implementation)")
     lib = _lib.load()
-    with torch.cuda.device(like.device):
+    with _lib.on(like.device):
         if workspace:
             nbytes = lib.sfa_cache_workspace_bytes(ctypes.byref(P))
             ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=like.device)
-            rc = getattr(lib, name)(ctypes.byref(P), ws.data_ptr(), nbytes, _stream(like))
+            rc = getattr(lib, name)(ctypes.byref(P), ws.data_ptr(), nbytes, _lib.stream_of(like.device))
         else:
-            rc = getattr(lib, name)(ctypes.byref(P), _stream(like))
+            rc = getattr(lib, name)(ctypes.byref(P), _lib.stream_of(like.device))
         _lib.check(rc, name)
 
 
@@ -155,8 +160,6 @@ def paged_cache_accept(pools: Sequence[torch.Tensor], block_table: torch.Tensor,
     keep = torch.empty_like(cache_seqlens)
     P = _params(None, block_table, cache_seqlens, page, num_pages, accepted if accepted.numel() else drafted, drafted, keep,
                 arr, accepted.shape[1])
-    if accepted.numel():
-        P.a_stride = accepted.stride(0)
     _call("sfa_cache_accept", P, block_table, workspace=False)
     return keep
 

@@ -79,7 +79,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 def _strides(x: torch.Tensor):
     """(batch, token, head) element strides of [B, T, H, D] or [T, H, D]."""
-    return (x.stride(0), x.stride(1), x.stride(2)) if x.dim() == 4 else (0, x.stride(0), x.stride(1))
+    s = x.stride()
+    return s[:3] if len(s) == 4 else (0, s[0], s[1])
 
 
 def _check(name: str, x: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
@@ -125,84 +126,82 @@ def _weight(name: str, w: Optional[torch.Tensor], x: torch.Tensor) -> Optional[t
         return None
     if w.dim() != 1 or w.shape[0] != x.shape[-1] or w.device != x.device or not w.is_floating_point():
         raise ValueError(f"{name} must be a floating-point vector of the head size on the inputs' device")
-    return w.float().contiguous()
+    return w if w.dtype == torch.float32 and w.is_contiguous() else w.float().contiguous()
 
 
-def _params(x: torch.Tensor, cfg: _Cfg, positions, frequencies) -> SfaRotaryParams:
-    P = SfaRotaryParams()
-    P.batch, P.len = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
-    P.dim, P.dtype = x.shape[-1], _DTYPE[x.dtype]
-    P.rot, P.start, P.interleaved = cfg.rot, cfg.start, 1 if cfg.interleaved else 0
-    P.eps, P.amplitude = cfg.eps, cfg.amplitude
-    if positions is not None:
-        P.positions, P.frequencies = positions.data_ptr(), frequencies.data_ptr()
-        P.pos64 = 1 if positions.dtype == torch.int64 else 0
-        P.p_sb, P.p_st = (positions.stride(0), positions.stride(1)) if positions.dim() == 2 else (0, positions.stride(0))
-    return P
+_pack = _lib.packer(SfaRotaryParams)
+_TURN, _PAGED = _lib.SFA_ROTARY_TURN, _lib.SFA_ROTARY_PAGED
+_NO_TENSOR = (0,) * 20
+_NO_CACHE = (0, 0, 0, 0)
 
 
-def _fill(t, x, w, turned: bool = True) -> None:
-    t.x, t.heads = x.data_ptr(), x.shape[-2]
-    t.x_sb, t.x_st, t.x_sh = _strides(x)
-    t.weight = None if w is None else w.data_ptr()
-    t.flags = _lib.SFA_ROTARY_TURN if turned else 0
+def _tensor(x, w, y=None, dy=None, dx=None, dw=None, turned=_TURN):
+    """The values of one SfaRotaryTensor."""
+    return (x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if dy is None else dy.data_ptr(),
+            0 if dx is None else dx.data_ptr(), 0 if w is None else w.data_ptr(), 0 if dw is None else dw.data_ptr(),
+            *_strides(x), *(_strides(y) if y is not None else (0, 0, 0)), *(_strides(dy) if dy is not None else (0, 0, 0)),
+            *(_strides(dx) if dx is not None else (0, 0, 0)), x.shape[-2], turned)
 
 
-def _stream(x: torch.Tensor) -> int:
-    return torch.cuda.current_stream(x.device).cuda_stream
+def _paged(x, w, pool, turned):
+    """The values of one SfaRotaryTensor that goes into a page pool."""
+    return (x.data_ptr(), pool.data_ptr(), 0, 0, 0 if w is None else w.data_ptr(), 0, *_strides(x), 0, pool.stride(1),
+            pool.stride(2), 0, 0, 0, 0, 0, 0, x.shape[-2], turned | _PAGED)
+
+
+def _params(x: torch.Tensor, tensors, cfg: _Cfg, positions, frequencies, cache=_NO_CACHE, sizes=_NO_CACHE) -> SfaRotaryParams:
+    batch, length = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
+    if positions is None:
+        pos, freq, sb, st, p64 = 0, 0, 0, 0, 0
+    else:
+        pos, freq, p64 = positions.data_ptr(), frequencies.data_ptr(), int(positions.dtype == torch.int64)
+        sb, st = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    n = len(tensors)
+    return _pack(*tensors[0], *(tensors[1] if n > 1 else _NO_TENSOR), *(tensors[2] if n > 2 else _NO_TENSOR), pos, freq,
+                 *cache, sb, st, n, batch, length, x.shape[-1], cfg.rot, cfg.start, int(cfg.interleaved), _DTYPE[x.dtype],
+                 p64, *sizes, cfg.eps, cfg.amplitude, 0)
 
 
 class _NormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, frequencies, cfg: _Cfg):
-        lib = _lib.load()
-        P = _params(q, cfg, positions, frequencies)
-        outs = []
-        for i, (x, w) in enumerate(((q, wq), (k, wk))):
-            if x is None:
-                break
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _fill(P.t[i], x, w)
-            P.t[i].y = y.data_ptr()
-            P.t[i].y_sb, P.t[i].y_st, P.t[i].y_sh = _strides(y)
-            outs.append(y)
-        P.num_tensors = len(outs)
-        with torch.cuda.device(q.device):
-            _lib.check(lib.sfa_rotary_fwd(ctypes.byref(P), _stream(q)), "sfa_rotary_fwd")
+        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        tensors = [_tensor(q, wq, oq)]
+        if k is not None:
+            ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            tensors.append(_tensor(k, wk, ok))
+        P = _params(q, tensors, cfg, positions, frequencies)
+        with _lib.on(q.device):
+            _lib.check(_lib.load().sfa_rotary_fwd(ctypes.byref(P), _lib.stream_of(q.device)), "sfa_rotary_fwd")
         ctx.save_for_backward(q, k, wq, wk, positions, frequencies)
         ctx.cfg = cfg
-        return tuple(outs) if k is not None else outs[0]
+        return (oq, ok) if k is not None else oq
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         q, k, wq, wk, positions, frequencies = ctx.saved_tensors
-        lib = _lib.load()
-        P = _params(q, ctx.cfg, positions, frequencies)
         need = ctx.needs_input_grad
         out = [None] * 7
-        held = []
-        n = 0
+        tensors, held = [], []
+        sums = False
         for i, (x, w) in enumerate(((q, wq), (k, wk))):
             if x is None or not (need[i] or need[2 + i]):
                 continue
             dy = _rows(grads[i])
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             dw = torch.empty_like(w) if w is not None and need[2 + i] else None
-            t = P.t[n]
-            _fill(t, x, w)
-            t.dy, t.dx, t.dweight = dy.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr()
-            t.dy_sb, t.dy_st, t.dy_sh = _strides(dy)
-            t.dx_sb, t.dx_st, t.dx_sh = _strides(dx)
+            tensors.append(_tensor(x, w, None, dy, dx, dw))
             out[i], out[2 + i] = dx, dw
             held.append(dy)
-            n += 1
-        P.num_tensors = n
-        if n:
-            with torch.cuda.device(q.device):
-                nbytes = lib.sfa_rotary_bwd_workspace_bytes(ctypes.byref(P))
-                ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
-                _lib.check(lib.sfa_rotary_bwd(ctypes.byref(P), ws.data_ptr(), nbytes, _stream(q)), "sfa_rotary_bwd")
+            sums = sums or dw is not None
+        if tensors:
+            lib, P, device = _lib.load(), _params(q, tensors, ctx.cfg, positions, frequencies), q.device
+            with _lib.on(device):
+                nbytes = lib.sfa_rotary_bwd_workspace_bytes(ctypes.byref(P)) if sums else 0
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+                _lib.check(lib.sfa_rotary_bwd(ctypes.byref(P), None if ws is None else ws.data_ptr(), nbytes,
+                                              _lib.stream_of(device)), "sfa_rotary_bwd")
         return tuple(out)
 
 
@@ -298,31 +297,20 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     cfg, positions, frequencies = _check_turn(q, positions, frequencies, interleaved, start, eps, amplitude)
     wq, wk = _weight("q_weight", q_weight, q), _weight("k_weight", k_weight, k)
     _need_cuda(q)
-    with torch.no_grad():
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
-        lens = cache_seqlens.contiguous()
-        cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        P = _params(q, cfg, positions, frequencies)
-        same = v.shape[-1] == q.shape[-1]
-        pools = ((P.t[1], k, wk, k_cache, True), (P.t[2], v, None, v_cache, False))
-        _fill(P.t[0], q, wq)
-        P.t[0].y = out.data_ptr()
-        P.t[0].y_sb, P.t[0].y_st, P.t[0].y_sh = _strides(out)
-        for t, x, w, c, turned in pools:
-            _fill(t, x, w, turned)
-            t.flags |= _lib.SFA_ROTARY_PAGED
-            t.y, t.y_sb, t.y_st, t.y_sh = c.data_ptr(), 0, c.stride(1), c.stride(2)
-        P.block_table, P.bt_stride, P.table_width = table.data_ptr(), table.stride(0), table.shape[1]
-        P.cache_seqlens, P.cu_seqlens = lens.data_ptr(), None if cu is None else cu.data_ptr()
-        P.num_seqs, P.num_pages, P.page_size = n, k_cache.shape[0], k_cache.shape[1]
-        P.num_tensors = 3 if same else 2
-        lib = _lib.load()
-        with torch.cuda.device(q.device):
-            if not same:                       # v's rows alone: its head size is another
-                V = SfaRotaryParams.from_buffer_copy(P)
-                V.t[0], V.num_tensors, V.dim, V.rot, V.start = P.t[2], 1, v.shape[-1], 0, 0
-                _lib.check(lib.sfa_rotary_fwd(ctypes.byref(V), _stream(q)), "sfa_rotary_fwd (append)")
-            _lib.check(lib.sfa_rotary_fwd(ctypes.byref(P), _stream(q)), "sfa_rotary_fwd (append)")
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
+    lens = cache_seqlens.contiguous()
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    cache = (table.data_ptr(), lens.data_ptr(), 0 if cu is None else cu.data_ptr(), table.stride(0))
+    sizes = (n, k_cache.shape[0], k_cache.shape[1], table.shape[1])
+    tensors = [_tensor(q, wq, out), _paged(k, wk, k_cache, _TURN), _paged(v, None, v_cache, 0)]
+    lib, stream = _lib.load(), _lib.stream_of(q.device)
+    with _lib.on(q.device):
+        if v.shape[-1] != q.shape[-1]:             # v's rows alone: their head size is another
+            V = _params(v, tensors[2:], _Cfg(0, 0, False, 0.0, 1.0), None, None, cache, sizes)
+            _lib.check(lib.sfa_rotary_fwd(ctypes.byref(V), stream), "sfa_rotary_fwd (append)")
+            tensors = tensors[:2]
+        P = _params(q, tensors, cfg, positions, frequencies, cache, sizes)
+        _lib.check(lib.sfa_rotary_fwd(ctypes.byref(P), stream), "sfa_rotary_fwd (append)")
     return out

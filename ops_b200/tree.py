@@ -13,8 +13,9 @@ import torch
 
 from . import _lib
 from ._lib import SfaTreeParams
-from .rotary import _check_pool, _check_table, _stream
+from .rotary import _check_pool, _check_table
 
+_pack = _lib.packer(SfaTreeParams)
 _DTYPE = {torch.bfloat16: _lib.SFA_DTYPE_BF16, torch.float16: _lib.SFA_DTYPE_F16}
 
 
@@ -84,28 +85,29 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("the inputs must be CUDA tensors (tree attention has no CPU implementation)")
     if max_seqlen_q is None:
         max_seqlen_q = int((cu_seqlens[1:] - cu_seqlens[:-1]).max().item()) if n else 0
-    with torch.no_grad(), torch.cuda.device(q.device):
-        q = q if _tma_ready(q) else q.clone(memory_format=torch.contiguous_format)
-        table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
-        lens = cache_seqlens.contiguous()
-        cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-        par = None if parents is None else parents.contiguous()
-        sink = None if attn_sink is None else attn_sink.float().contiguous()
-        o = torch.empty(total, q.shape[1], v_cache.shape[3], dtype=q.dtype, device=q.device)
-        lse = torch.empty(total, q.shape[1], dtype=torch.float32, device=q.device)
-        P = SfaTreeParams(
-            q=q.data_ptr(), k=k_cache.data_ptr(), v=v_cache.data_ptr(), block_table=table.data_ptr(),
-            cache_seqlens=lens.data_ptr(), cu_seqlens=None if cu is None else cu.data_ptr(),
-            parents=None if par is None else par.data_ptr(), attn_sink=None if sink is None else sink.data_ptr(),
-            o=o.data_ptr(), lse=lse.data_ptr(), q_st=q.stride(0), q_sh=q.stride(1), k_st=k_cache.stride(1),
-            k_sh=k_cache.stride(2), v_st=v_cache.stride(1), v_sh=v_cache.stride(2), o_st=o.stride(0), o_sh=o.stride(1),
-            l_st=lse.stride(0), l_sh=lse.stride(1), bt_stride=table.stride(0), num_seqs=n, total_q=total,
-            max_q=int(max_seqlen_q), max_k=int(max_seqlen_k) if max_seqlen_k is not None
-            else min(2**31 - 1, table.shape[1] * k_cache.shape[1]), h_q=q.shape[1], h_kv=k_cache.shape[2],
-            d_qk=q.shape[2], d_v=v_cache.shape[3], num_pages=k_cache.shape[0], page_size=k_cache.shape[1],
-            table_width=table.shape[1], dtype=_DTYPE[q.dtype], scale=float(scale))
-        lib = _lib.load()
-        nbytes = lib.sfa_tree_workspace_bytes(ctypes.byref(P))          # 0 also when the call is refused
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
-        _lib.check(lib.sfa_tree_attention(ctypes.byref(P), ws.data_ptr(), nbytes, _stream(q)), "sfa_tree_attention")
+    device = q.device
+    q = q if _tma_ready(q) else q.detach().clone(memory_format=torch.contiguous_format)
+    table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
+    lens = cache_seqlens.contiguous()
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    par = None if parents is None else parents.contiguous()
+    sink = None if attn_sink is None else attn_sink.detach().float().contiguous()
+    hq, dv = q.shape[1], v_cache.shape[3]
+    o = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
+    lse = torch.empty(total, hq, dtype=torch.float32, device=device)
+    pages, page, hk = k_cache.shape[:3]
+    ks, vs = k_cache.stride(), v_cache.stride()
+    width = table.shape[1]
+    if max_seqlen_k is None:
+        max_seqlen_k = min(2**31 - 1, width * page)
+    P = _pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),
+              0 if cu is None else cu.data_ptr(), 0 if par is None else par.data_ptr(),
+              0 if sink is None else sink.data_ptr(), o.data_ptr(), lse.data_ptr(), q.stride(0), q.stride(1), ks[1], ks[2],
+              vs[1], vs[2], hq * dv, dv, hq, 1, table.stride(0), n, total, int(max_seqlen_q), int(max_seqlen_k), hq, hk,
+              q.shape[2], dv, pages, page, width, _DTYPE[q.dtype], float(scale), 0)
+    lib, at = _lib.load(), ctypes.byref(P)
+    with _lib.on(device):
+        nbytes = lib.sfa_tree_workspace_bytes(at)                       # 0 also when the call is refused
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        _lib.check(lib.sfa_tree_attention(at, ws.data_ptr(), nbytes, _lib.stream_of(device)), "sfa_tree_attention")
     return o, lse
