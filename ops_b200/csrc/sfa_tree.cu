@@ -33,49 +33,18 @@
 // Warps: 0 K (and Q, key masks), 1 V, 2 MMA issue (one thread), 4-7 softmax.
 // Every wait is bounded (~2 s); on expiry the kernel records (7 << 16) | site in
 // the status word and returns.
-#include "sfa_common.cuh"
-#include "sfa_internal.h"
-#include "sfa_tc_common.cuh"
-#include "sfa_tc_host.h"
-#include "sfa_tok_common.cuh"
+#include "sfa_tree.cuh"
 
 #include <algorithm>
 #include <string>
 
 namespace sfa {
-using namespace tc;
-using namespace tok;
-
 namespace tree {
 
 constexpr int kThreads = 256;
 constexpr int kKeys = 64;                       // keys per chunk
 constexpr int kSlab = kKeys * 128;              // bytes of a 64-key x 64-dim slab
-constexpr int kQSlab = 128 * 128;               // bytes of a 128-row x 64-dim Q slab
-constexpr int kMaxNodes = SFA_TREE_MAX_NODES;
-constexpr int kAncWords = kMaxNodes / 32 + 3;   // + 2 zero words behind, odd row stride
 constexpr int kMasks = 8;                       // key-mask ring: more chunks than stages in flight
-constexpr float kRescaleLog2 = 8.f;
-
-struct Args {
-  SfaTreeParams p;
-  int G;             // query heads per kv head
-  int GB, NT;        // heads and drafted rows of a tile
-  int n_hg;          // head tiles (G above 128)
-  int ntiles;        // row tiles = gridDim.y
-  int ranges;        // gridDim.x
-  int min_chunks;    // chunks of a range at least
-  int nkq, nkv;      // 64-dim slabs of a key / value row
-  int dvp;           // d_v rounded up to 16
-  int box;           // rows of a K / V box
-  int kst, vst;      // ring stages
-  uint32_t col_s, tmem_cols;
-  uint32_t off_k, off_v, off_sh;
-  float* part_o;     // [range][tile][2][dvp / 4][128][4]
-  float2* part_ml;   // [range][tile][2][128]  (m, l)
-  int32_t* cum;      // [num_seqs + 1] chunks before each sequence
-  int32_t* status;
-};
 
 struct Shared {
   uint64_t q_full, q_empty;
@@ -88,84 +57,23 @@ struct Shared {
   uint32_t bad[2];                     // keys of the chunk whose value row has a non-finite element
   uint2 mask[kMasks];                  // keys of the chunk that exist
   int scan[kThreads / 32];
-  int start_s, start_h, start_c, left; // this CTA's range
+  Range range;
   short parent[kMaxNodes];
   uint32_t anc[128][kAncWords];        // ancestors of each row of the tile
 };
 
+constexpr int kId = 7;                          // of this kernel in the status word
 __device__ __forceinline__ bool wt(uint64_t* bar, uint32_t parity, int32_t* status, int site) {
-  if (mbar_wait(bar, parity)) return true;
-  record_status(status, (7 << 16) | site);
-  return false;
+  return bounded_wait(bar, parity, status, kId, site);
 }
 __device__ __forceinline__ bool wtw(uint64_t* bar, uint32_t parity, int32_t* status, int site) {
   return __all_sync(0xffffffffu, wt(bar, parity, status, site));
 }
 
-// A sequence: its drafted rows [q0, q0 + rows), cache length, cache rows before the drafted ones
-// (negative when the cache is shorter), positions the table covers, 64-key chunks of those.
-struct Seq {
-  int q0, rows, prefix, kvc, nch;
-};
-
-__device__ __forceinline__ Seq load_seq(const SfaTreeParams& p, int s) {
-  Seq r;
-  const int len = __ldg(p.cache_seqlens + s);
-  if (p.cu_seqlens) {
-    r.q0 = __ldg(p.cu_seqlens + s);
-    r.rows = max(0, __ldg(p.cu_seqlens + s + 1) - r.q0);
-  } else {
-    r.q0 = s;
-    r.rows = 1;
-  }
-  r.prefix = len - r.rows;
-  const int64_t covered = (int64_t)p.table_width * p.page_size;
-  r.kvc = (int)max((int64_t)0, min((int64_t)len, covered));
-  r.nch = (r.kvc + kKeys - 1) / kKeys;
-  return r;
-}
-
-// A piece of this CTA's range: chunks [c0, c1) of unit (s, h); whole: the unit lies in this range.
-struct Piece {
-  int s, h, c0, c1;
-  bool whole;
-  Seq q;
-};
-
-struct Walk {
-  const SfaTreeParams* p;
-  int s, h, c, left;
-  Seq q;
-  __device__ __forceinline__ Walk(const SfaTreeParams& pp, const Shared& S)
-      : p(&pp), s(S.start_s), h(S.start_h), c(S.start_c), left(S.left) {
-    if (left > 0) q = load_seq(pp, s);
-  }
-  __device__ __forceinline__ bool next(Piece& g) {
-    if (left <= 0) return false;
-    const int n = min(q.nch - c, left);
-    g.s = s; g.h = h; g.c0 = c; g.c1 = c + n;
-    g.whole = n == q.nch;
-    g.q = q;
-    left -= n;
-    c = 0;
-    if (left > 0 && ++h == p->h_kv) {
-      h = 0;
-      do { q = load_seq(*p, ++s); } while (q.nch == 0);   // left > 0: a later sequence has chunks
-    }
-    return true;
-  }
-};
-
-// First drafted row of the tile, and its chunks: those that hold a key one of the tile's rows can see.
+// Cuts the piece to the chunks of the tile's rows.
 __device__ __forceinline__ void clip_to_tile(const Args& a, int tile, Piece& g, int& node0) {
-  node0 = (tile / a.n_hg) * a.NT;
-  if (node0 >= g.q.rows) {
-    g.c1 = g.c0;
-    return;
-  }
-  const int last = g.q.prefix + min(g.q.rows, node0 + a.NT);          // keys below it
-  const int kend = max(0, min(g.q.kvc, last));
-  g.c1 = max(g.c0, min(g.c1, (kend + kKeys - 1) / kKeys));
+  node0 = node_of_tile(a, tile);
+  g.c1 = tile_end(a, tile, g);
 }
 
 // The chunks of the tile's pieces one after another.
@@ -175,7 +83,7 @@ struct Chunks {
   const Args* a;
   int c, node0;
   bool first;
-  __device__ __forceinline__ Chunks(const Args& aa, const Shared& S) : w(aa.p, S), a(&aa), c(0), node0(0), first(false) {
+  __device__ __forceinline__ Chunks(const Args& aa, const Shared& S) : w(aa, S.range), a(&aa), c(0), node0(0), first(false) {
     g.c0 = g.c1 = 0;
   }
   __device__ __forceinline__ bool next(int tile) {
@@ -194,14 +102,6 @@ struct Chunks {
   }
   __device__ __forceinline__ bool last() const { return c + 1 == g.c1; }
 };
-
-// Pool row of the box at cache position pos, -1 if it holds no key.
-__device__ __forceinline__ int box_row(const SfaTreeParams& p, const Piece& g, int pos) {
-  if (pos >= g.q.kvc) return -1;
-  const int pg = __ldg(p.block_table + (int64_t)g.s * p.bt_stride + pos / p.page_size);
-  if (pg < 0 || pg >= p.num_pages) return -1;
-  return pg * p.page_size + pos % p.page_size;
-}
 
 // Producer of one ring (K or V): boxes of every chunk, in order.  The table
 // entries of a chunk are read while the one before waits for its stage.
@@ -272,26 +172,6 @@ __device__ __forceinline__ void produce(const Args& a, Shared& S, uint8_t* ring,
   }
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  return pack_bf16x2(lo, hi);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Whether one of the two 16-bit values of w is infinite or NaN, per half.
-template <typename T>
-__device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == (e << 16) ? 0xffff0000u : 0u);
-}
-__device__ __forceinline__ float as_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float as_f(__half x) { return __half2float(x); }
-
 // The softmax warps' own barrier (bounded, unlike a named barrier).
 __device__ __forceinline__ bool meet(Shared& S, int& n, int32_t* status) {
   warp_arrive(&S.sync);
@@ -307,7 +187,7 @@ __device__ __forceinline__ void softmax_warps(const Args& a, Shared& S, uint8_t*
   const int my_node = a.n_hg > 1 ? 0 : m / a.GB;              // drafted row of this thread in the tile
   const int my_head = a.n_hg > 1 ? (tile % a.n_hg) * 128 + m : m % a.GB;
   const bool in_tile = my_node < a.NT && my_head < a.G;
-  Walk w(p, S);
+  Walk w(a, S.range);
   Piece g;
   int ci = 0, meets = 0, added = 0;
   bool ok = true;
@@ -335,19 +215,7 @@ __device__ __forceinline__ void softmax_warps(const Args& a, Shared& S, uint8_t*
       if (!(ok = meet(S, meets, a.status))) break;            // the piece before is done with both
       for (int i = m; i < rows; i += 128) S.parent[i] = (short)max(-1, min(__ldg(p.parents + g.q.q0 + i), i));
       if (!(ok = meet(S, meets, a.status))) break;
-      if (m < a.NT) {
-        uint32_t* anc = S.anc[m];
-        for (int i = 0; i < kAncWords; ++i) anc[i] = 0;
-        int n = node0 + m;
-        if (n < rows) {
-          while (true) {                                      // ends: n falls with every step
-            anc[n >> 5] |= 1u << (n & 31);
-            const int up = S.parent[n];
-            if (up < 0 || up >= n) break;
-            n = up;
-          }
-        }
-      }
+      if (m < a.NT) mark_ancestors(S.anc[m], S.parent, node0 + m, rows);
       if (!(ok = meet(S, meets, a.status))) break;
     }
     float mref = -INFINITY, l = 0.f;
@@ -361,23 +229,9 @@ __device__ __forceinline__ void softmax_warps(const Args& a, Shared& S, uint8_t*
       const bool whole = (km.x & km.y) == 0xffffffffu && !drafted;
       uint32_t lo = km.x, hi = km.y;
       if (drafted) {
-        uint64_t vis;
-        const int j = node - d0;                              // the row's own key in the chunk
-        if (p.parents == nullptr) {
-          vis = j < 0 ? 0ull : j >= 63 ? ~0ull : (2ull << j) - 1;
-        } else if (d0 >= 0) {
-          const uint32_t* anc = S.anc[my_node];
-          const int wd = d0 >> 5, sh = d0 & 31;
-          const uint32_t w0 = wd < kAncWords ? anc[wd] : 0, w1 = wd + 1 < kAncWords ? anc[wd + 1] : 0,
-                         w2 = wd + 2 < kAncWords ? anc[wd + 2] : 0;
-          vis = (uint64_t)__funnelshift_r(w0, w1, sh) | ((uint64_t)__funnelshift_r(w1, w2, sh) << 32);
-        } else {
-          const int sh = -d0;                                 // 1 .. 63 keys before the drafted ones
-          const uint32_t* anc = S.anc[my_node];
-          vis = (((uint64_t)anc[1] << 32 | anc[0]) << sh) | ((1ull << sh) - 1);
-        }
-        lo &= (uint32_t)vis;
-        hi &= (uint32_t)(vis >> 32);
+        const bool by_tree = p.parents != nullptr;
+        lo &= sees32(S.anc[my_node], by_tree, node, d0);
+        hi &= sees32(S.anc[my_node], by_tree, node, d0 + 32);
       }
       if (!live) lo = hi = 0;
       const uint32_t ts = tl + a.col_s + sb * kKeys;
@@ -520,7 +374,7 @@ __device__ __forceinline__ void softmax_warps(const Args& a, Shared& S, uint8_t*
     if (!any) continue;
     const int head = g.h * a.G + my_head;
     if (split) {
-      const int64_t slot = ((int64_t)blockIdx.x * a.ntiles + tile) * 2 + (begins ? 1 : 0);
+      const int64_t slot = part_slot(a, blockIdx.x, tile, begins);
       if (live) a.part_ml[slot * 128 + m] = make_float2(mref, l);
       if (ran) {
         float4* dst = reinterpret_cast<float4*>(a.part_o) + slot * (a.dvp / 4) * 128 + m;
@@ -570,7 +424,7 @@ __device__ __forceinline__ void softmax_warps(const Args& a, Shared& S, uint8_t*
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
 tree_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
             const __grid_constant__ CUtensorMap tmv) {
   extern __shared__ uint8_t smem_raw[];
@@ -597,7 +451,6 @@ tree_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap 
     }
     mbar_init(&S.pv_done, 1);
     mbar_init(&S.sync, 4);
-    S.left = 0;
     fence_barrier_init();
     prefetch_tmap(&tmq);
     prefetch_tmap(&tmk);
@@ -607,42 +460,7 @@ tree_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap 
     tmem_alloc(&S.tmem_base, a.tmem_cols);
     tmem_relinquish();
   }
-  // this CTA's range: chunks before each sequence by a block scan, every thread a strip of sequences
-  const int n = p.num_seqs, strip = (n + kThreads - 1) / kThreads;
-  const int s0 = min(n, (int)threadIdx.x * strip), s1 = min(n, s0 + strip);
-  int mine = 0;
-  for (int s = s0; s < s1; ++s) mine += load_seq(p, s).nch;
-  int run = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += up;
-  }
-  if (lane == 31) S.scan[warp] = run;
-  __syncthreads();
-  int before = run - mine, all = 0;
-  for (int i = 0; i < kThreads / 32; ++i) {
-    if (i < warp) before += S.scan[i];
-    all += S.scan[i];
-  }
-  const int line = all * p.h_kv;
-  const int len = max(a.min_chunks, (line + a.ranges - 1) / a.ranges);
-  const int64_t x0 = (int64_t)blockIdx.x * len;
-  const bool writer = blockIdx.x == 0 && blockIdx.y == 0;
-  for (int s = s0; s < s1; ++s) {
-    const int nch = load_seq(p, s).nch;
-    if (writer) a.cum[s] = before;
-    const int64_t u0 = (int64_t)before * p.h_kv;
-    if (x0 >= u0 && x0 < u0 + (int64_t)nch * p.h_kv) {
-      const int off = (int)(x0 - u0);
-      S.start_s = s;
-      S.start_h = off / nch;
-      S.start_c = off % nch;
-      S.left = (int)min((int64_t)len, (int64_t)line - x0);
-    }
-    before += nch;
-  }
-  if (writer && threadIdx.x == 0) a.cum[n] = all;
+  find_range(a, S);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -657,9 +475,8 @@ tree_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap 
     if (lane == 0) {
       // S of a chunk is issued before PV of the one before; both run in issue order, so S may
       // overwrite the buffer whose P the PV before that reads
-      const uint32_t typ = __is_same(T, __half) ? (1u << 7) | (1u << 10) : 0u;    // A / B format bits of fp16 are 0
-      const uint32_t id_s = idesc_bf16(128, kKeys, false, false) ^ typ;
-      const uint32_t id_o = idesc_bf16(128, a.dvp, false, true) ^ typ;
+      const uint32_t id_s = idesc_bf16(128, kKeys, false, false) ^ type_bits<T>();
+      const uint32_t id_o = idesc_bf16(128, a.dvp, false, true) ^ type_bits<T>();
       Chunks it(a, S);
       bool ok = true;
       int qi = 0;
@@ -758,7 +575,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int u0 = c0 * p.h_kv + h * nch;
   const int r0 = u0 / len, r1 = nch > 0 ? (u0 + nch - 1) / len : r0;
   if (nch > 0 && r0 == r1) return;
-  const Seq q = load_seq(p, s);
+  const Seq q = load_seq(a, s);
   const int node0 = tile / a.n_hg * a.NT;
   for (int i = first; i < tile_rows * groups; i += step) {
     const int m = i % tile_rows, grp = i / tile_rows;
@@ -771,7 +588,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
       empty_row(row, head, grp);
       continue;
     }
-    auto slot = [&](int r) { return ((int64_t)r * a.ntiles + tile) * 2 + (r == r0 ? 1 : 0); };
+    auto slot = [&](int r) { return part_slot(a, r, tile, r == r0); };
     const float s2 = p.attn_sink ? __ldg(p.attn_sink + head) * kLog2e : -INFINITY;
     float M = s2;
     for (int r = r0; r <= r1; ++r) M = fmaxf(M, a.part_ml[slot(r) * 128 + m].x);
@@ -802,6 +619,7 @@ struct Plan {
   size_t smem;
   size_t off_ml, off_cum, ws;
   int tile_rows;      // rows of a tile that can be live
+  bool pair;          // the pair kernel
 };
 
 static int bad(const std::string& m) { return report_error(SFA_ERR_INVALID_ARGUMENT, "tree attention: " + m); }
@@ -842,8 +660,23 @@ static int check(const SfaTreeParams* p) {
   return SFA_OK;
 }
 
-// Shapes, shared memory and the split.  Two CTAs share an SM when both rings fit twice with two stages
-// each and O fits beside two S buffers in 256 TMEM columns.
+// Ring stages that fit `budget` bytes of shared memory, K first; false if two of each do not.
+static bool fit_rings(Args& a, size_t budget, size_t fixed, size_t kb, size_t vb) {
+  a.kst = a.vst = 2;
+  if (fixed + 2 * kb + 2 * vb > budget) return false;
+  while (a.kst < 4 || a.vst < 4) {
+    const size_t now = fixed + a.kst * kb + a.vst * vb;
+    if (a.kst <= a.vst && a.kst < 4 && now + kb <= budget) ++a.kst;
+    else if (a.vst < 4 && now + vb <= budget) ++a.vst;
+    else break;
+  }
+  return true;
+}
+
+// Shapes, kernel, shared memory and the split.  The pair kernel (128-key chunks, two softmax
+// warpgroups) takes every shape whose O fits twice beside two 128-key S tiles in TMEM (d_v <= 128) and
+// whose rings fit shared memory: 128 rows of d_qk = d_v = 128 over 131072 keys take 1.7 times as long
+// in the single kernel, which keeps the wider heads.
 static Plan make_plan(const SfaTreeParams& p) {
   Plan pl{};
   Args& a = pl.a;
@@ -858,32 +691,44 @@ static Plan make_plan(const SfaTreeParams& p) {
   a.nkq = (p.d_qk + 63) / 64;
   a.nkv = (p.d_v + 63) / 64;
   a.dvp = (p.d_v + 15) / 16 * 16;
-  a.box = 1;
-  while (a.box < kKeys && p.page_size % (a.box * 2) == 0) a.box *= 2;
-  const size_t sh = (sizeof(Shared) + 127) / 128 * 128, q = (size_t)a.nkq * kQSlab;
-  const size_t kb = (size_t)a.nkq * kSlab, vb = (size_t)a.nkv * kSlab;
-  const size_t half = 113 * 1024 - 1024, full = 226 * 1024 - 1024;
-  const bool two = a.dvp <= 128 && q + 2 * kb + 2 * vb + sh <= half;
-  const size_t budget = two ? half : full;
-  a.kst = a.vst = 2;
-  while (a.kst < 4) {
-    const size_t now = q + a.kst * kb + a.vst * vb + sh;
-    if (a.vst < a.kst && now + vb <= budget) ++a.vst;
-    else if (a.vst == a.kst && now + kb <= budget) ++a.kst;
-    else break;
+  const size_t q = (size_t)a.nkq * kQSlab, full = 226 * 1024 - 1024;
+  size_t sh = (pair_shared_bytes() + 127) / 128 * 128;
+  int ctas_y = a.ntiles;
+  if (a.dvp <= 128) {
+    const size_t kb = (size_t)a.nkq * 128 * 128, vb = (size_t)a.nkv * 128 * 128;
+    a.two = a.ntiles > 1 && fit_rings(a, full, 2 * q + sh, kb, vb);
+    pl.pair = a.two || fit_rings(a, full, q + sh, kb, vb);
   }
-  if (a.vst < a.kst && q + a.kst * kb + (a.vst + 1) * vb + sh <= budget) ++a.vst;
-  a.col_s = a.dvp <= 128 ? 128 : 256;
-  a.tmem_cols = two ? 256 : 512;
-  a.off_k = (uint32_t)q;
-  a.off_v = a.off_k + (uint32_t)(a.kst * kb);
-  a.off_sh = a.off_v + (uint32_t)(a.vst * vb);
-  pl.smem = a.off_sh + sh + 1024;
-  if (!two) pl.smem = std::max(pl.smem, (size_t)116 * 1024);   // all TMEM columns: one CTA per SM
-  a.min_chunks = 2;
+  if (pl.pair) {
+    a.keys = 128;
+    a.off_k = (uint32_t)(a.two ? 2 * q : q);
+    a.off_v = a.off_k + (uint32_t)(a.kst * a.nkq * 128 * 128);
+    a.off_sh = a.off_v + (uint32_t)(a.vst * a.nkv * 128 * 128);
+    a.tmem_cols = 512;
+    a.min_chunks = 1;
+    if (a.two) ctas_y = (a.ntiles + 1) / 2;
+  } else {
+    a.keys = kKeys;
+    sh = (sizeof(Shared) + 127) / 128 * 128;
+    const size_t kb = (size_t)a.nkq * kSlab, vb = (size_t)a.nkv * kSlab;
+    fit_rings(a, full, q + sh, kb, vb);           // 256 dims: 64 KB of Q, 32 KB a stage
+    a.off_k = (uint32_t)q;
+    a.off_v = a.off_k + (uint32_t)(a.kst * kb);
+    a.off_sh = a.off_v + (uint32_t)(a.vst * vb);
+    a.col_s = a.dvp <= 128 ? 128 : 256;
+    a.tmem_cols = 512;
+    a.min_chunks = 2;
+  }
+  a.box = 1;
+  while (a.box < a.keys && p.page_size % (a.box * 2) == 0) {
+    a.box *= 2;
+    ++a.box_log;
+  }
+  // all TMEM columns: one CTA per SM
+  pl.smem = std::max(a.off_sh + sh + 1024, (size_t)116 * 1024);
   const int64_t covered = std::min<int64_t>((int64_t)p.table_width * p.page_size, std::max(1, p.max_k));
-  const int64_t line = std::max<int64_t>(1, (int64_t)p.num_seqs * p.h_kv * ((covered + kKeys - 1) / kKeys));
-  const int64_t slots = (int64_t)device_sm_count() * (two ? 2 : 1) / a.ntiles;
+  const int64_t line = std::max<int64_t>(1, (int64_t)p.num_seqs * p.h_kv * ((covered + a.keys - 1) / a.keys));
+  const int64_t slots = (int64_t)device_sm_count() / ctas_y;
   a.ranges = (int)std::max<int64_t>(1, std::min(slots, (line + a.min_chunks - 1) / a.min_chunks));
   const size_t pieces = a.ranges > 1 ? (size_t)a.ranges * a.ntiles * 2 : 0;
   size_t off = pieces * 128 * a.dvp * sizeof(float);
@@ -901,11 +746,15 @@ static cudaError_t launch(Plan& pl, const CUtensorMap& tq, const CUtensorMap& tk
   cudaError_t e = cudaSuccess;
   const bool keys = a.p.num_seqs > 0 && a.p.num_pages > 0 && a.p.table_width > 0;
   if (keys) {
-    e = cudaFuncSetAttribute(tree_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
+    if (pl.pair) {
+      if ((e = launch_pair(a, pl.smem, tq, tk, tv, st)) != cudaSuccess) return e;
+    } else {
+      e = cudaFuncSetAttribute(tree_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
     if (e != cudaSuccess) return e;
     tree_kernel<T><<<dim3(a.ranges, a.ntiles), kThreads, pl.smem, st>>>(a, tq, tk, tv);
     note_launch("tree_attention", st);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
   } else {
     // no keys at all: every sequence has zero chunks
     if ((e = cudaMemsetAsync(a.cum, 0, ((size_t)a.p.num_seqs + 1) * sizeof(int32_t), st)) != cudaSuccess) return e;

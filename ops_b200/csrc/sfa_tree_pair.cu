@@ -1,0 +1,799 @@
+// sfa_tree_pair.cu — the tree attention of sfa_tree.cu with two softmax
+// warpgroups per CTA (d_v <= 128).
+//
+// A warpgroup's work between two MMAs (read S, maximum, exponentials, P back to
+// TMEM) takes about as long as the MMAs and their hand-overs, so two of them take
+// turns on the tensor core: each has its own S and O in TMEM (2 x 128 + 2 x 128
+// columns) and works on chunks of 128 keys, the width at which the MMAs run at
+// full rate.  What the two share depends on the rows:
+//   rows: two row tiles (256 rows) against the same chunk, which is loaded once
+//         for both: large trees, bound by the exponentials;
+//   keys: one row tile, alternate chunks; the two (m, l, O) are joined at the end
+//         of the piece out of TMEM: decoding and small trees, bound by reads.
+// A CTA goes by piece: it falls back to `keys` where its second tile is empty.
+//
+// Warps: 0 K, Q and key masks; 1 V; 2 MMA issue (one thread); 3 clears value rows
+// that must not enter a product (see scrub); 4-7 and 8-11 softmax.
+// Every wait is bounded (~2 s); on expiry the kernel records (8 << 16) | site in
+// the status word and returns.
+#include "sfa_tree.cuh"
+
+namespace sfa {
+namespace tree {
+namespace pair {
+
+constexpr int kThreads = 384;
+constexpr int kKeys = 128;
+constexpr int kSlab = kKeys * 128;   // bytes of a 128-key x 64-dim slab
+constexpr int kRing = 8;             // key masks and scrub results: more chunks than are in flight
+constexpr uint32_t kColS = 256;      // S of warpgroup w at 256 + 128 w, its O at 128 w
+constexpr int kId = 8;
+
+struct Shared {
+  uint64_t q_full, q_empty;
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t scrub_go[kRing], v_ready[kRing];
+  uint64_t s_full[2], p_full[2], pv_done[2], meet[2];
+  uint64_t b_ready, b_free;            // keys: warpgroup B's piece is complete / has been taken
+  uint32_t tmem_base;
+  uint32_t zeroed[2];                  // O of a piece was initialised by the warpgroup
+  uint32_t bad[kRing][4];              // keys whose value row has a non-finite element
+  uint4 mask[kRing];                   // keys of the chunk that exist
+  uint32_t word[kRing];                // chunk_word of the chunk
+  float2 ml[128];                      // warpgroup B's (m, l)
+  int scan[kThreads / 32];
+  Range range;
+  short parent[2][kMaxNodes];
+  uint32_t anc[2][128][kAncWords];     // ancestors of each row of the warpgroup's tile
+};
+
+__device__ __forceinline__ bool wt(uint64_t* bar, uint32_t parity, int32_t* status, int site) {
+  return bounded_wait(bar, parity, status, kId, site);
+}
+__device__ __forceinline__ bool wtw(uint64_t* bar, uint32_t parity, int32_t* status, int site) {
+  return __all_sync(0xffffffffu, wt(bar, parity, status, site));
+}
+
+// A piece as this CTA's two tiles see it: chunks [c0, end), of which tile A (rows: B) needs those
+// before end_a (end_b), and those from `scrub` on hold value rows to clear.
+struct Job {
+  Piece g;
+  int c0, end, end_a, end_b, scrub;
+  bool rows;
+};
+
+__device__ __forceinline__ Job make_job(const Args& a, const Piece& g) {
+  Job j;
+  j.g = g;
+  j.c0 = g.c0;
+  const int ta = a.two ? 2 * blockIdx.y : blockIdx.y;
+  j.end_a = tile_end(a, ta, g);
+  j.rows = a.two && ta + 1 < a.ntiles && node_of_tile(a, ta + 1) < g.q.rows;
+  j.end_b = j.rows ? tile_end(a, ta + 1, g) : g.c0;
+  j.end = max(j.end_a, j.end_b);
+  // the last, partly filled chunk; every chunk with drafted keys when some rows do not see some of them
+  int f = g.q.kvc % kKeys ? g.q.nch - 1 : g.q.nch;
+  if (g.q.rows > 1) f = min(f, max(0, g.q.prefix) / kKeys);
+  j.scrub = max(f, g.c0);
+  return j;
+}
+
+// The chunks of the CTA's jobs one after another; n counts them, k those that are scrubbed.
+struct Chunks {
+  Walk w;
+  Job j;
+  int c, n, k;
+  __device__ __forceinline__ Chunks(const Args& a, const Shared& S) : w(a, S.range), c(0), n(-1), k(-1) { j.c0 = j.end = 0; }
+  __device__ __forceinline__ bool next() {
+    if (c + 1 < j.end) {
+      ++c;
+    } else {
+      do {
+        Piece g;
+        if (!w.next(g)) return false;
+        j = make_job(*w.a, g);
+      } while (j.c0 >= j.end);
+      c = j.c0;
+    }
+    ++n;
+    k += scrubbed();
+    return true;
+  }
+  __device__ __forceinline__ bool first() const { return c == j.c0; }
+  __device__ __forceinline__ bool last() const { return c + 1 == j.end; }
+  __device__ __forceinline__ bool scrubbed() const { return c >= j.scrub; }
+  // the warpgroups that work on the chunk, as bits
+  __device__ __forceinline__ int groups() const {
+    return j.rows ? (c < j.end_a ? 1 : 0) | (c < j.end_b ? 2 : 0) : 1 << ((c - j.c0) & 1);
+  }
+};
+
+// What the MMA issuer has to know of a chunk, in a word: the warpgroups that work on it, those for
+// which it is the first / last of the job, whether it opens / ends the job (Q), is scrubbed, and reads
+// Q's second tile; kStop ends the kernel.
+enum : uint32_t {
+  kGroups = 3u, kBegins = 3u << 2, kEnds = 3u << 4, kOpens = 1u << 6, kCloses = 1u << 7, kScrubbed = 1u << 8, kRows = 1u << 9,
+  kStop = 1u << 31
+};
+__device__ __forceinline__ uint32_t chunk_word(const Chunks& it) {
+  const Job& j = it.j;
+  const uint32_t groups = it.groups();
+  uint32_t ends;
+  if (j.rows) ends = (it.c + 1 == j.end_a ? 1u : 0u) | (it.c + 1 == j.end_b ? 2u : 0u);
+  else ends = it.c + 2 >= j.end ? 3u : 0u;
+  const uint32_t begins = (j.rows ? it.first() : it.c < j.c0 + 2) ? 3u : 0u;
+  return groups | begins << 2 | ends << 4 | (it.first() ? kOpens : 0u) | (it.last() ? kCloses : 0u) |
+         (it.scrubbed() ? kScrubbed : 0u) | (j.rows ? kRows : 0u);
+}
+
+// Producer of the K ring (which also loads Q and writes the key masks and chunk words) or of the V ring.
+// One function for both, and no loop unrolled: what the warps of a CTA run has to stay in the
+// instruction cache together.
+__device__ __forceinline__ void produce(const Args& a, Shared& S, bool is_k, uint8_t* ring, uint8_t* sq,
+                                        const CUtensorMap* map, const CUtensorMap* tmq) {
+  const SfaTreeParams& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int slabs = is_k ? a.nkq : a.nkv, stages = is_k ? a.kst : a.vst;
+  const int nb_log = 7 - a.box_log, nb = 1 << nb_log;      // boxes of a chunk, 1 .. 128
+  const int outside = p.num_pages * p.page_size;           // a row past the pool: zeros
+  uint64_t* full = is_k ? S.k_full : S.v_full;
+  uint64_t* empty = is_k ? S.k_empty : S.v_empty;
+  Chunks it(a, S);
+  bool ok = true;
+  int qi = 0, st = 0, phase = 1;
+  while (ok && it.next()) {
+    const int n = it.n, h = it.j.g.h, k0 = it.c * kKeys, left = it.j.g.q.kvc - k0;
+    // the lane's box (the first of its boxes when there are more than 32)
+    int row = box_row(p, it.j.g, k0 + ((lane & (nb - 1)) << a.box_log));
+    if (is_k && it.first()) {
+      if (lane == 0 && (ok = wt(&S.q_empty, (qi & 1) ^ 1, a.status, 1))) {
+        const int tiles = it.j.rows ? 2 : 1;
+        mbar_arrive_expect_tx(&S.q_full, (uint32_t)(tiles * a.nkq * a.GB * a.NT * 128));
+        int tile = a.two ? 2 * blockIdx.y : blockIdx.y;
+#pragma unroll 1
+        for (int x = 0; x < tiles * a.nkq; ++x) {
+          const int s = x < a.nkq ? x : x - a.nkq;
+          if (x == a.nkq) ++tile;
+          tma_load_4d(sq + x * kQSlab, tmq, &S.q_full, s * 64, h * a.G + (tile % a.n_hg) * 128,
+                      it.j.g.q.q0 + node_of_tile(a, tile), 0);
+        }
+      }
+      ++qi;
+    }
+    if (lane == 0 && ok) ok = wt(&empty[st], phase, a.status, is_k ? 2 : 3);
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    if (!ok) break;
+    uint4 mask = make_uint4(~0u, ~0u, ~0u, ~0u);
+    const bool there = __all_sync(0xffffffffu, row >= 0) && left >= kKeys && nb <= 32;
+    if (is_k) {
+      if (!there) {
+        uint32_t m[4];
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int key = 32 * i + lane;
+          const uint32_t w = __ballot_sync(0xffffffffu, key < left && box_row(p, it.j.g, k0 + (key >> a.box_log << a.box_log)) >= 0);
+          if (i == 0) m[0] = w;
+          else if (i == 1) m[1] = w;
+          else if (i == 2) m[2] = w;
+          else m[3] = w;
+        }
+        mask = make_uint4(m[0], m[1], m[2], m[3]);
+      }
+      if (lane == 0) {
+        S.mask[n % kRing] = mask;
+        S.word[n % kRing] = chunk_word(it);
+      }
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(slabs * kSlab));
+    __syncwarp();
+    uint8_t* dst = ring + (size_t)st * slabs * kSlab;
+#pragma unroll 1
+    for (int i = lane; i < nb * slabs; i += 32) {
+      const int b = i & (nb - 1), s = i >> nb_log;
+      if (nb > 32) row = box_row(p, it.j.g, k0 + (b << a.box_log));
+      tma_load_4d(dst + s * kSlab + (b << a.box_log) * 128, map, &full[st], s * 64, row >= 0 ? row : outside, h, 0);
+    }
+    if (!is_k && it.scrubbed() && lane == 0) mbar_arrive(&S.scrub_go[it.k % kRing]);
+    if (++st == stages) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+  if (is_k && ok && lane == 0 && wt(&empty[st], phase, a.status, 2)) {
+    S.word[(it.n + 1) % kRing] = kStop;
+    mbar_arrive(&full[st]);
+  }
+}
+
+// Value rows that must not enter a product.  Rows behind the cache are cleared (a stale row's NaN
+// would turn 0 * NaN into NaN); of drafted rows, which not all query rows see, non-finite elements
+// are cleared and noted, and the softmax warps add them to the rows that see them.
+template <typename T>
+__device__ __forceinline__ void scrub(const Args& a, Shared& S, uint8_t* sv) {
+  const int lane = threadIdx.x & 31;
+  Chunks it(a, S);
+  bool ok = true;
+  while (ok && it.next()) {
+    if (!it.scrubbed()) continue;
+    const int slot = it.k % kRing, vs = it.n % a.vst;
+    // the producer has passed the stage's use before: its barrier is in this use's phase
+    if (!(ok = wtw(&S.scrub_go[slot], (it.k / kRing) & 1, a.status, 4))) break;
+    if (!(ok = wtw(&S.v_full[vs], (it.n / a.vst) & 1, a.status, 5))) break;
+    const int k0 = it.c * kKeys, left = it.j.g.q.kvc - k0, drafted = it.j.g.q.rows > 1 ? it.j.g.q.prefix - k0 : kKeys;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const int key = lane + 32 * i;
+      bool found = false;
+      if (key >= left || key >= drafted) {
+#pragma unroll 1
+        for (int s = 0; s < a.nkv; ++s) {
+          uint4* row = reinterpret_cast<uint4*>(sv + ((size_t)vs * a.nkv + s) * kSlab + key * 128);
+#pragma unroll 2
+          for (int x = 0; x < 8; ++x) {
+            if (key >= left) {
+              row[x] = make_uint4(0, 0, 0, 0);
+            } else {
+              const uint4 v = row[x];
+              const uint32_t b0 = nonfinite2<T>(v.x), b1 = nonfinite2<T>(v.y), b2 = nonfinite2<T>(v.z),
+                             b3 = nonfinite2<T>(v.w);
+              if (b0 | b1 | b2 | b3) {
+                found = true;
+                row[x] = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+              }
+            }
+          }
+        }
+      }
+      const uint32_t f = __ballot_sync(0xffffffffu, found);
+      if (lane == 0) S.bad[slot][i] = f;
+    }
+    fence_proxy_async_smem();
+    warp_arrive(&S.v_ready[slot]);
+  }
+}
+
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The issuing thread takes what is ready: PV of the oldest task whose P is there, then S of the next
+// chunk for a warpgroup that has no P outstanding (S overwrites the columns of P, and MMAs run in issue
+// order, so it goes behind the PV that reads P, and right behind it: a warpgroup waits for both).
+__device__ __forceinline__ void issue(const Args& a, Shared& S, uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t tmem,
+                                      uint32_t types) {
+  const uint32_t id_s = idesc_bf16(128, kKeys, false, false) ^ types;
+  const uint32_t id_o = idesc_bf16(128, a.dvp, false, true) ^ types;
+  const uint32_t k_step = (uint32_t)(a.nkq * kSlab) >> 4, v_step = (uint32_t)(a.nkv * kSlab) >> 4;
+  const uint32_t q_tile = (uint32_t)(a.nkq * kQSlab) >> 4;
+  const uint64_t q0 = smem_desc(smem_u32(sq), 16, 1024, kSw128), k0 = smem_desc(smem_u32(sk), 16, 1024, kSw128);
+  const uint64_t v0 = smem_desc(smem_u32(sv), kSlab, 1024, kSw128);
+  const int tail = (a.p.d_qk - (a.nkq - 1) * 64 + 15) / 16;      // 16-dim steps of the last slab
+  uint32_t waiting = 0;                                          // warpgroups whose P is outstanding
+  uint32_t sw = 0, rest_s = 0, pw = 0, rest_p = 0;               // words of the chunks at hand, warpgroups left of them
+  uint32_t ks = 0, kph = 0, vs = 0, vph = 0, nq = 0, np[2] = {0, 0};
+  uint32_t cs = 0, cp = 0, scrubs = 0;                           // chunks begun by S / by PV, scrubbed ones passed
+  bool stop = false;
+  uint64_t idle_since = 0;
+  uint32_t spins = 0;
+  while (true) {
+    bool moved = false;
+    if (rest_p == 0 && cp < cs) {
+      pw = S.word[cp++ % kRing];
+      rest_p = pw & kGroups;
+    }
+    if (rest_p != 0) {
+      const uint32_t wg = (rest_p & 1u) ? 0u : 1u;
+      const bool opens = rest_p == (pw & kGroups);
+      if (((waiting >> wg) & 1u) && ready(&S.p_full[wg], np[wg] & 1u) &&
+          (!opens || (ready(&S.v_full[vs], vph) &&
+                      (!(pw & kScrubbed) || ready(&S.v_ready[scrubs % kRing], (scrubs / kRing) & 1u))))) {
+        tc_fence_after();
+        ++np[wg];
+        if (opens && (pw & kScrubbed)) ++scrubs;
+        const uint32_t add = !((pw & kBegins) >> 2 >> wg & 1u) || *(volatile uint32_t*)&S.zeroed[wg] != 0;
+        const uint32_t pa = tmem + kColS + 128 * wg, d = tmem + 128 * wg;
+        const uint64_t vd = v0 + vs * v_step;
+        mma_bf16_ts(d, pa, vd, id_o, add);
+#pragma unroll
+        for (int i = 1; i < kKeys / 16; ++i) mma_bf16_ts(d, pa + i * 8, vd + (uint32_t)(i * (2048 >> 4)), id_o, 1);
+        waiting &= ~(1u << wg);
+        rest_p &= ~(1u << wg);
+        if (rest_p == 0) {
+          mma_commit(&S.v_empty[vs]);
+          if (++vs == (uint32_t)a.vst) {
+            vs = 0;
+            vph ^= 1u;
+          }
+        }
+        if (((pw & kEnds) >> 4 >> wg) & 1u) mma_commit(&S.pv_done[wg]);
+        moved = true;
+      }
+    }
+    if (rest_s != 0) {
+      const uint32_t wg = (rest_s & 1u) ? 0u : 1u;
+      const bool opens = (sw & kOpens) != 0 && rest_s == (sw & kGroups);
+      if (!((waiting >> wg) & 1u) && (!opens || ready(&S.q_full, nq & 1u))) {
+        tc_fence_after();
+        nq += opens ? 1u : 0u;
+        const uint32_t d = tmem + kColS + 128 * wg;
+        uint64_t qx = q0 + (((sw & kRows) && wg) ? q_tile : 0u), kx = k0 + ks * k_step;
+        uint32_t add = 0;
+#pragma unroll 1
+        for (int x = a.nkq; x > 1; --x) {
+          mma_bf16_ss(d, qx, kx, id_s, add);
+          mma_bf16_ss(d, qx + 2, kx + 2, id_s, 1);
+          mma_bf16_ss(d, qx + 4, kx + 4, id_s, 1);
+          mma_bf16_ss(d, qx + 6, kx + 6, id_s, 1);
+          qx += kQSlab >> 4;
+          kx += kSlab >> 4;
+          add = 1;
+        }
+        mma_bf16_ss(d, qx, kx, id_s, add);
+        if (tail > 1) mma_bf16_ss(d, qx + 2, kx + 2, id_s, 1);
+        if (tail > 2) mma_bf16_ss(d, qx + 4, kx + 4, id_s, 1);
+        if (tail > 3) mma_bf16_ss(d, qx + 6, kx + 6, id_s, 1);
+        mma_commit(&S.s_full[wg]);
+        waiting |= 1u << wg;
+        rest_s &= ~(1u << wg);
+        if (rest_s == 0) {
+          mma_commit(&S.k_empty[ks]);
+          if (++ks == (uint32_t)a.kst) {
+            ks = 0;
+            kph ^= 1u;
+          }
+          if (sw & kCloses) mma_commit(&S.q_empty);
+        }
+        moved = true;
+      }
+    }
+    if (!stop && rest_s == 0 && ready(&S.k_full[ks], kph)) {
+      sw = S.word[cs % kRing];
+      stop = (sw & kStop) != 0;
+      rest_s = stop ? 0u : sw & kGroups;
+      cs += stop ? 0u : 1u;
+      moved = true;
+    }
+    if (moved) {
+      idle_since = 0;
+      continue;
+    }
+    if (stop && rest_p == 0 && cp == cs) return;
+    if ((++spins & 63) != 0) continue;
+    const uint64_t now = global_timer_ns();
+    if (idle_since == 0) {
+      idle_since = now;
+    } else if (now - idle_since > kWaitLimitNs) {
+      record_status(a.status, (kId << 16) | 6);
+      return;
+    }
+  }
+}
+
+// 32 lanes x 32 columns; the registers hold them after ld_wait32.
+__device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+               : "r"(taddr));
+}
+
+// Waits for this thread's TMEM loads and makes their registers depend on it.
+__device__ __forceinline__ void ld_wait32(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                 "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+
+// Two fp32 lanes in one instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void untwo(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_packed(float& word, float f);
+template <>
+__device__ __forceinline__ void scale_packed<__nv_bfloat16>(float& word, float f) {
+  const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&word));
+  word = __uint_as_float(pack2<__nv_bfloat16>(v.x * f, v.y * f));
+}
+template <>
+__device__ __forceinline__ void scale_packed<__half>(float& word, float f) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&word));
+  word = __uint_as_float(pack2<__half>(v.x * f, v.y * f));
+}
+
+// O (o_cols columns) and P (p_cols columns of packed pairs) times fac, in TMEM.
+template <typename T>
+__device__ __noinline__ void rescale(uint32_t to, int o_cols, uint32_t tp, int p_cols, float fac) {
+#pragma unroll 1
+  for (int y = 0; y < o_cols; y += 16) {
+    float o[16];
+    tmem_ld16(to + y, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] *= fac;
+    tmem_st16(to + y, o);
+  }
+#pragma unroll 1
+  for (int y = 0; y < p_cols; y += 16) {
+    float o[16];
+    tmem_ld16(tp + y, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) scale_packed<T>(o[k], fac);
+    tmem_st16(tp + y, o);
+  }
+  tmem_st_wait();
+}
+
+template <typename T>
+__device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32_t tmem) {
+  const SfaTreeParams& p = a.p;
+  const int m = threadIdx.x & 127, wq = m >> 5;
+  const uint32_t tl = tmem + ((uint32_t)(wq * 32) << 16), to = tl + 128 * wg, ts = tl + kColS + 128 * wg;
+  const float c2 = p.scale * kLog2e;
+  const uint64_t c22 = two(c2, c2);
+  const bool by_tree = p.parents != nullptr;
+  Walk walk(a, S.range);
+  Piece g;
+  int n = 0, jobs = 0, met = 0, joined = 0, base = 0, scrubs = 0;   // tasks, ended pieces, meetings, joins; chunks and scrubs before the job
+  bool ok = true, owe = false;
+  auto meet = [&](int site) {
+    warp_arrive(&S.meet[wg]);
+    return wtw(&S.meet[wg], (met++) & 1, a.status, site);
+  };
+  while (ok && walk.next(g)) {
+    const Job j = make_job(a, g);
+    const int tile = (a.two ? 2 * blockIdx.y : blockIdx.y) + (j.rows ? wg : 0);
+    const int node0 = node_of_tile(a, tile);
+    const int my_node = a.n_hg > 1 ? 0 : m / a.GB;
+    const int my_head = a.n_hg > 1 ? (tile % a.n_hg) * 128 + m : m % a.GB;
+    const int node = node0 + my_node;
+    const bool live = my_node < a.NT && my_head < a.G && node < g.q.rows && g.q.q0 + node < p.total_q;
+    const bool any = __any_sync(0xffffffffu, live);
+    const int prefix = g.q.prefix;
+    const int c_first = j.rows ? j.c0 : j.c0 + wg, c_end = j.rows ? (wg ? j.end_b : j.end_a) : j.end, c_step = j.rows ? 1 : 2;
+    const bool ran = c_first < c_end;
+    if (by_tree && ran && c_end * kKeys > prefix) {
+      const int rows = min(g.q.rows, min(kMaxNodes, p.total_q - g.q.q0));
+      if (!(ok = meet(11))) break;                            // the piece before is done with both
+#pragma unroll 1
+      for (int i = m; i < rows; i += 128) S.parent[wg][i] = (short)max(-1, min(__ldg(p.parents + g.q.q0 + i), i));
+      if (!(ok = meet(12))) break;
+      if (m < a.NT) mark_ancestors(S.anc[wg][m], S.parent[wg], node0 + m, rows);
+      if (!(ok = meet(13))) break;
+    }
+    float mref = -INFINITY, l = 0.f;
+    for (int c = c_first; c < c_end; c += c_step, ++n) {
+      const int cn = base + (c - j.c0);
+      const bool first = c == c_first;
+      if (!(ok = wtw(&S.s_full[wg], n & 1, a.status, 14))) break;
+      tc_fence_after();
+      // S of this chunk was issued behind PV of the warpgroup's last one: O may be changed from here on
+      const uint4 km = S.mask[cn % kRing];
+      const int d0 = c * kKeys - prefix;                      // the chunk's first key, as a drafted row
+      const bool drafted = d0 + kKeys > 0;
+      const bool whole = (km.x & km.y & km.z & km.w) == ~0u && !drafted;
+      uint32_t vis[4] = {km.x, km.y, km.z, km.w};
+      if (any) {
+        if (drafted) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vis[i] &= sees32(S.anc[wg][my_node], by_tree, node, d0 + 32 * i);
+        }
+        uint64_t sum0 = 0, sum1 = 0;
+        // 64 keys at a time in a loop that is not unrolled: with the 128 keys unrolled the softmax, issue
+        // and producer loops together miss the instruction cache on every pass (a third of all stalls:
+        // 515 us against 323 for 8 trees of 64 nodes at 32 keys a pass)
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          float s[2][32];
+          ld32(ts + 64 * i, s[0]);
+          ld32(ts + 64 * i + 32, s[1]);
+          ld_wait32(s[0]);
+          ld_wait32(s[1]);
+          if (!whole) {
+            const uint32_t v0 = !live ? 0u : i ? vis[2] : vis[0], v1 = !live ? 0u : i ? vis[3] : vis[1];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (!((v0 >> k) & 1u)) s[0][k] = -INFINITY;
+              if (!((v1 >> k) & 1u)) s[1][k] = -INFINITY;
+            }
+          }
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = fmaxf(s[0][k], s[1][k]);
+#pragma unroll
+          for (int k = 8; k < 32; ++k) x[k & 7] = fmaxf(x[k & 7], fmaxf(s[0][k], s[1][k]));
+          const float top =
+              fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * c2;
+          const bool up = live && (top > mref + kRescaleLog2 || (mref == -INFINITY && top > -INFINITY));
+          if (__any_sync(0xffffffffu, up)) {
+            float fac = 1.f;
+            if (up) {
+              if (mref != -INFINITY) fac = ex2(mref - top);
+              mref = top;
+            }
+            if (__any_sync(0xffffffffu, fac != 1.f)) {
+              // rare: O, the sums and this chunk's P so far to the raised maximum
+              const uint64_t f2 = two(fac, fac);
+              sum0 = fma2(sum0, f2, 0ull);
+              sum1 = fma2(sum1, f2, 0ull);
+              l *= fac;
+              rescale<T>(to, first ? 0 : a.dvp, ts, 32 * i, fac);
+            }
+          }
+          const float nm = mref == -INFINITY ? 0.f : -mref;   // nothing seen yet: any reference gives p = 0
+          const uint64_t nm2 = two(nm, nm);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float pk[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float p0, p1;
+              untwo(fma2(two(s[h][k], s[h][k + 1]), c22, nm2), p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              if (k & 2) sum1 = add2(sum1, two(p0, p1));
+              else sum0 = add2(sum0, two(p0, p1));
+              pk[k / 2] = __uint_as_float(pack2<T>(p0, p1));
+            }
+            tmem_st16(ts + 32 * i + 16 * h, pk);              // over columns of S that have been read
+          }
+        }
+        float s0, s1;
+        untwo(add2(sum0, sum1), s0, s1);
+        l += s0 + s1;
+        tmem_st_wait();
+      }
+      if (first) {
+        if (m == 0) S.zeroed[wg] = 0;
+        if (owe) {                                            // warpgroup A has taken O of the piece before
+          if (!(ok = wtw(&S.b_free, (joined - 1) & 1, a.status, 15))) break;
+          owe = false;
+        }
+      }
+      if (drafted && g.q.rows > 1) {
+        const int k = scrubs + (c - j.scrub);
+        if (!(ok = wtw(&S.v_ready[k % kRing], (k / kRing) & 1, a.status, 16))) break;
+        const uint32_t* bad = S.bad[k % kRing];
+        if (bad[0] | bad[1] | bad[2] | bad[3]) {
+          // non-finite elements that the scrub took out of V, for the rows that see them
+          tc_fence_after();
+          if (first) {
+            const float z[16] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int y = 0; y < a.dvp; y += 16) tmem_st16(to + y, z);
+            tmem_st_wait();
+            if (m == 0) S.zeroed[wg] = 1;
+          }
+#pragma unroll 1
+          for (int b = 0; b < kKeys; ++b) {
+            if (!((bad[b >> 5] >> (b & 31)) & 1u)) continue;
+            const uint32_t mine = b < 32 ? vis[0] : b < 64 ? vis[1] : b < 96 ? vis[2] : vis[3];
+            const bool sees = live && ((mine >> (b & 31)) & 1u);
+            const int row = box_row(p, g, c * kKeys + b);
+            const T* v = static_cast<const T*>(p.v) + (int64_t)max(row, 0) * p.v_st + (int64_t)g.h * p.v_sh;
+#pragma unroll 1
+            for (int y = 0; y < a.dvp; y += 16) {
+              float o[16];
+              tmem_ld16(to + y, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float e = sees && y + i < p.d_v ? as_f(v[y + i]) : 0.f;
+                if (!isfinite(e)) o[i] += e;
+              }
+              tmem_st16(to + y, o);
+            }
+            tmem_st_wait();
+          }
+        }
+      }
+      tc_fence_before();
+      warp_arrive(&S.p_full[wg]);
+    }
+    if (!ok) break;
+    base += j.end - j.c0;
+    scrubs += max(0, j.end - j.scrub);
+    if (ran) {
+      if (!(ok = wtw(&S.pv_done[wg], (jobs++) & 1, a.status, 17))) break;
+      tc_fence_after();
+    }
+    float wa = 1.f, wb = 0.f;
+    const bool join = !j.rows && j.end - j.c0 > 1;            // both warpgroups hold a part of the rows
+    if (!j.rows && wg == 1) {
+      if (join) {
+        S.ml[m] = make_float2(mref, l);
+        tc_fence_before();
+        warp_arrive(&S.b_ready);
+        owe = true;
+        ++joined;
+      }
+      continue;
+    }
+    if (join) {
+      if (!(ok = wtw(&S.b_ready, (joined++) & 1, a.status, 18))) break;
+      tc_fence_after();
+      const float2 b = S.ml[m];
+      const float M = fmaxf(mref, b.x);
+      wa = mref == -INFINITY ? 0.f : ex2(mref - M);
+      wb = b.x == -INFINITY ? 0.f : ex2(b.x - M);
+      // a NaN sum has to survive a weight of zero
+      l = (mref == -INFINITY ? l : l * wa) + (b.x == -INFINITY ? b.y : b.y * wb);
+      mref = M;
+    }
+    if (any) {
+      const int head = g.h * a.G + my_head;
+      const bool split = !g.whole;
+      const bool none = mref == -INFINITY && l == 0.f;
+      float fa = wa, fb = wb;
+      float4* dst = nullptr;
+      T* orow = nullptr;
+      if (split) {
+        const int64_t slot = part_slot(a, blockIdx.x, tile, g.c0 == 0);
+        if (live) a.part_ml[slot * 128 + m] = make_float2(mref, l);
+        dst = reinterpret_cast<float4*>(a.part_o) + slot * (a.dvp / 4) * 128 + m;
+      } else {
+        const float sink = p.attn_sink && live ? __ldg(p.attn_sink + head) : -INFINITY;
+        const float s2 = sink * kLog2e, M = fmaxf(mref, s2);
+        const float w = mref == -INFINITY ? 0.f : ex2(mref - M);
+        const float lt = l * w + (s2 == -INFINITY ? 0.f : ex2(s2 - M));
+        const float inv = none ? 0.f : w / lt;
+        fa *= inv;
+        fb *= inv;
+        const int64_t row = g.q.q0 + node;
+        orow = static_cast<T*>(p.o) + row * p.o_st + (int64_t)head * p.o_sh;
+        if (live) p.lse[row * p.l_st + (int64_t)head * p.l_sh] = none ? sink : (M + lg2(lt)) * kLn2;
+      }
+#pragma unroll 1
+      for (int y = 0; y < a.dvp; y += 16) {
+        float o[16];
+        if (ran) {
+          tmem_ld16(to + y, o);
+          tmem_ld_wait();
+        }
+        if (join) {
+          float ob[16];
+          tmem_ld16(tl + 128 + y, ob);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = (fa == 0.f ? 0.f : o[i] * fa) + (fb == 0.f ? 0.f : ob[i] * fb);
+        } else if (ran) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= fa;
+        }
+        if (none || !ran) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0.f;
+        }
+        if (live) {
+          if (split) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[(y / 4 + i) * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+              if (y + i < p.d_v)
+                *reinterpret_cast<uint4*>(orow + y + i) =
+                    make_uint4(pack2<T>(o[i], o[i + 1]), pack2<T>(o[i + 2], o[i + 3]), pack2<T>(o[i + 4], o[i + 5]),
+                               pack2<T>(o[i + 6], o[i + 7]));
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    if (join) warp_arrive(&S.b_free);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_pair_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                 const __grid_constant__ CUtensorMap tmv) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sk = sq + a.off_k;
+  uint8_t* sv = sq + a.off_v;
+  Shared& S = *reinterpret_cast<Shared*>(sq + a.off_sh);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    mbar_init(&S.q_full, 1);
+    mbar_init(&S.q_empty, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&S.k_full[i], 1);
+      mbar_init(&S.k_empty[i], 1);
+      mbar_init(&S.v_full[i], 1);
+      mbar_init(&S.v_empty[i], 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&S.scrub_go[i], 1);
+      mbar_init(&S.v_ready[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.p_full[i], 4);
+      mbar_init(&S.pv_done[i], 1);
+      mbar_init(&S.meet[i], 4);
+    }
+    mbar_init(&S.b_ready, 4);
+    mbar_init(&S.b_free, 4);
+    fence_barrier_init();
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
+  }
+  if (warp == 2) {
+    tmem_alloc(&S.tmem_base, a.tmem_cols);
+    tmem_relinquish();
+  }
+  find_range(a, S);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem_base;
+  if (warp < 2) {
+    produce(a, S, warp == 0, warp == 0 ? sk : sv, sq, warp == 0 ? &tmk : &tmv, &tmq);
+  } else if (warp == 2) {
+    if ((threadIdx.x & 31) == 0) issue(a, S, sq, sk, sv, tmem, type_bits<T>());
+  } else if (warp == 3) {
+    scrub<T>(a, S, sv);
+  } else {
+    softmax<T>(a, S, (warp - 4) >> 2, tmem);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, a.tmem_cols);
+}
+
+}  // namespace pair
+
+size_t pair_shared_bytes() { return sizeof(pair::Shared); }
+
+template <typename T>
+static cudaError_t launch_pair_typed(const Args& a, size_t smem, const CUtensorMap& tq, const CUtensorMap& tk,
+                                     const CUtensorMap& tv, cudaStream_t st) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(pair::tree_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int y = a.two ? (a.ntiles + 1) / 2 : a.ntiles;
+  pair::tree_pair_kernel<T><<<dim3(a.ranges, y), pair::kThreads, smem, st>>>(a, tq, tk, tv);
+  note_launch("tree_attention_pair", st);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pair(const Args& a, size_t smem, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        cudaStream_t st) {
+  return a.p.dtype == SFA_DTYPE_F16 ? launch_pair_typed<__half>(a, smem, tq, tk, tv, st)
+                                    : launch_pair_typed<__nv_bfloat16>(a, smem, tq, tk, tv, st);
+}
+
+}  // namespace tree
+}  // namespace sfa
