@@ -701,6 +701,7 @@ static Plan make_plan(const SfaTreeParams& p) {
   }
   if (pl.pair) {
     a.keys = 128;
+    a.keys_log = 7;
     a.off_k = (uint32_t)(a.two ? 2 * q : q);
     a.off_v = a.off_k + (uint32_t)(a.kst * a.nkq * 128 * 128);
     a.off_sh = a.off_v + (uint32_t)(a.vst * a.nkv * 128 * 128);
@@ -709,6 +710,7 @@ static Plan make_plan(const SfaTreeParams& p) {
     if (a.two) ctas_y = (a.ntiles + 1) / 2;
   } else {
     a.keys = kKeys;
+    a.keys_log = 6;
     sh = (sizeof(Shared) + 127) / 128 * 128;
     const size_t kb = (size_t)a.nkq * kSlab, vb = (size_t)a.nkv * kSlab;
     fit_rings(a, full, q + sh, kb, vb);           // 256 dims: 64 KB of Q, 32 KB a stage

@@ -28,7 +28,7 @@ struct Args {
   int GB, NT;        // heads and drafted rows of a tile
   int n_hg;          // head tiles (G above 128)
   int ntiles;        // row tiles
-  int keys;          // keys per chunk
+  int keys, keys_log; // keys per chunk, a power of two
   int two;           // pair kernel: a CTA takes two row tiles
   int ranges;        // gridDim.x
   int min_chunks;    // chunks of a range at least
@@ -64,7 +64,7 @@ static __device__ __noinline__ Seq load_seq(const Args& a, int s) {
   r.prefix = len - r.rows;
   const int64_t covered = (int64_t)p.table_width * p.page_size;
   r.kvc = (int)max((int64_t)0, min((int64_t)len, covered));
-  r.nch = (r.kvc + a.keys - 1) / a.keys;
+  r.nch = (r.kvc + a.keys - 1) >> a.keys_log;
   return r;
 }
 
@@ -140,13 +140,16 @@ struct Walk {
     c = 0;
     if (left > 0 && ++h == a->p.h_kv) {
       h = 0;
-      do { q = load_seq(*a, ++s); } while (q.nch == 0);   // left > 0: a later sequence has chunks
+      do { q = load_seq(*a, ++s); } while (q.nch == 0 && s + 1 < a->p.num_seqs);   // left > 0: a later one has chunks
+      if (q.nch == 0) left = 0;
     }
     return true;
   }
 };
 
-__device__ __forceinline__ int node_of_tile(const Args& a, int tile) { return (tile / a.n_hg) * a.NT; }
+__device__ __forceinline__ int node_of_tile(const Args& a, int tile) {
+  return (a.n_hg == 1 ? tile : tile / a.n_hg) * a.NT;
+}
 
 // End of the piece's chunks that hold a key one of the tile's rows can see (c0 if the tile has no rows).
 __device__ __forceinline__ int tile_end(const Args& a, int tile, const Piece& g) {
@@ -154,7 +157,7 @@ __device__ __forceinline__ int tile_end(const Args& a, int tile, const Piece& g)
   if (node0 >= g.q.rows) return g.c0;
   const int last = g.q.prefix + min(g.q.rows, node0 + a.NT);          // keys below it
   const int kend = max(0, min(g.q.kvc, last));
-  return max(g.c0, min(g.c1, (kend + a.keys - 1) / a.keys));
+  return max(g.c0, min(g.c1, (kend + a.keys - 1) >> a.keys_log));
 }
 
 // A wait of at most ~2 s; on expiry the status word gets the kernel and the site.
@@ -219,6 +222,13 @@ template <typename T>
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == (e << 16) ? 0xffff0000u : 0u);
+}
+// Whether one of them is: an exponent of all ones carries into the sign's place.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return (((w & e) + one) & 0x80008000u) != 0;
 }
 __device__ __forceinline__ float as_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_f(__half x) { return __half2float(x); }

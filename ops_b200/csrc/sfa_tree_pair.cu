@@ -27,6 +27,7 @@ constexpr int kKeys = 128;
 constexpr int kSlab = kKeys * 128;   // bytes of a 128-key x 64-dim slab
 constexpr int kRing = 8;             // key masks and scrub results: more chunks than are in flight
 constexpr uint32_t kColS = 256;      // S of warpgroup w at 256 + 128 w, its O at 128 w
+constexpr float kMost = 16384.f;     // of P: far inside fp16, and sums of it far inside fp32
 constexpr int kId = 8;
 
 struct Shared {
@@ -37,7 +38,7 @@ struct Shared {
   uint64_t b_ready, b_free;            // keys: warpgroup B's piece is complete / has been taken
   uint32_t tmem_base;
   uint32_t zeroed[2];                  // O of a piece was initialised by the warpgroup
-  uint32_t bad[kRing][4];              // keys whose value row has a non-finite element
+  alignas(16) uint32_t bad[kRing][4];              // keys whose value row has a non-finite element
   uint4 mask[kRing];                   // keys of the chunk that exist
   uint32_t word[kRing];                // chunk_word of the chunk
   float2 ml[128];                      // warpgroup B's (m, l)
@@ -62,7 +63,7 @@ struct Job {
   bool rows;
 };
 
-__device__ __forceinline__ Job make_job(const Args& a, const Piece& g) {
+static __device__ __noinline__ Job make_job(const Args& a, const Piece& g) {
   Job j;
   j.g = g;
   j.c0 = g.c0;
@@ -220,39 +221,51 @@ __device__ __forceinline__ void scrub(const Args& a, Shared& S, uint8_t* sv) {
     if (!(ok = wtw(&S.scrub_go[slot], (it.k / kRing) & 1, a.status, 4))) break;
     if (!(ok = wtw(&S.v_full[vs], (it.n / a.vst) & 1, a.status, 5))) break;
     const int k0 = it.c * kKeys, left = it.j.g.q.kvc - k0, drafted = it.j.g.q.rows > 1 ? it.j.g.q.prefix - k0 : kKeys;
+    if (lane < 4) S.bad[slot][lane] = 0;
+    __syncwarp();
+    // four rows at a time, eight lanes a row (a 16-byte group each)
+    uint8_t* at = sv + (size_t)vs * a.nkv * kSlab + (lane & 7) * 16;
 #pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      const int key = lane + 32 * i;
+    for (int r = max(0, min(left, drafted)) & ~3; r < kKeys; r += 4) {
+      const int key = r + (lane >> 3);
       bool found = false;
-      if (key >= left || key >= drafted) {
-#pragma unroll 1
-        for (int s = 0; s < a.nkv; ++s) {
-          uint4* row = reinterpret_cast<uint4*>(sv + ((size_t)vs * a.nkv + s) * kSlab + key * 128);
 #pragma unroll 2
-          for (int x = 0; x < 8; ++x) {
-            if (key >= left) {
-              row[x] = make_uint4(0, 0, 0, 0);
-            } else {
-              const uint4 v = row[x];
-              const uint32_t b0 = nonfinite2<T>(v.x), b1 = nonfinite2<T>(v.y), b2 = nonfinite2<T>(v.z),
-                             b3 = nonfinite2<T>(v.w);
-              if (b0 | b1 | b2 | b3) {
-                found = true;
-                row[x] = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
-              }
-            }
+      for (int s = 0; s < a.nkv; ++s) {
+        uint4* x = reinterpret_cast<uint4*>(at + s * kSlab + key * 128);
+        if (key >= left) {
+          *x = make_uint4(0, 0, 0, 0);
+        } else if (key >= drafted) {
+          const uint4 v = *x;
+          if (any_nonfinite2<T>(v.x) | any_nonfinite2<T>(v.y) | any_nonfinite2<T>(v.z) | any_nonfinite2<T>(v.w)) {
+            found = true;
+            *x = make_uint4(v.x & ~nonfinite2<T>(v.x), v.y & ~nonfinite2<T>(v.y), v.z & ~nonfinite2<T>(v.z),
+                            v.w & ~nonfinite2<T>(v.w));
           }
         }
       }
       const uint32_t f = __ballot_sync(0xffffffffu, found);
-      if (lane == 0) S.bad[slot][i] = f;
+      if (f != 0 && lane == 0)
+        S.bad[slot][r >> 5] |= ((f & 0xffu ? 1u : 0u) | (f & 0xff00u ? 2u : 0u) | (f & 0xff0000u ? 4u : 0u) |
+                                (f & 0xff000000u ? 8u : 0u)) << (r & 31);
     }
     fence_proxy_async_smem();
     warp_arrive(&S.v_ready[slot]);
   }
 }
 
-// Whether the phase has completed, without waiting.
+// One lane of the converged warp.  Around MMAs the warp stays converged and their operands are uniform,
+// so that they sit in uniform registers: an MMA issued from a branch on the lane number takes three
+// times the code (the compiler makes every operand uniform first), and the kernel lives or dies by
+// its instruction cache.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ uint64_t desc(uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; }
+
+// Whether the phase has completed, without waiting; one answer for the warp.
 __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -262,10 +275,10 @@ __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) {
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return ok != 0;
+  return __all_sync(0xffffffffu, ok != 0);
 }
 
-// The issuing thread takes what is ready: PV of the oldest task whose P is there, then S of the next
+// The issuing warp takes what is ready: PV of the oldest task whose P is there, then S of the next
 // chunk for a warpgroup that has no P outstanding (S overwrites the columns of P, and MMAs run in issue
 // order, so it goes behind the PV that reads P, and right behind it: a warpgroup waits for both).
 __device__ __forceinline__ void issue(const Args& a, Shared& S, uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t tmem,
@@ -274,47 +287,55 @@ __device__ __forceinline__ void issue(const Args& a, Shared& S, uint8_t* sq, uin
   const uint32_t id_o = idesc_bf16(128, a.dvp, false, true) ^ types;
   const uint32_t k_step = (uint32_t)(a.nkq * kSlab) >> 4, v_step = (uint32_t)(a.nkv * kSlab) >> 4;
   const uint32_t q_tile = (uint32_t)(a.nkq * kQSlab) >> 4;
-  const uint64_t q0 = smem_desc(smem_u32(sq), 16, 1024, kSw128), k0 = smem_desc(smem_u32(sk), 16, 1024, kSw128);
-  const uint64_t v0 = smem_desc(smem_u32(sv), kSlab, 1024, kSw128);
+  // descriptors: addresses advance in the low word, the high word holds layout only
+  const uint64_t dq = smem_desc(smem_u32(sq), 16, 1024, kSw128), dk = smem_desc(smem_u32(sk), 16, 1024, kSw128);
+  const uint64_t dv = smem_desc(smem_u32(sv), kSlab, 1024, kSw128);
+  const uint32_t q0 = uniform((uint32_t)dq), k0 = uniform((uint32_t)dk), v0 = uniform((uint32_t)dv);
+  const uint32_t hi_k = uniform((uint32_t)(dk >> 32)), hi_v = uniform((uint32_t)(dv >> 32));
+  tmem = uniform(tmem);
   const int tail = (a.p.d_qk - (a.nkq - 1) * 64 + 15) / 16;      // 16-dim steps of the last slab
   uint32_t waiting = 0;                                          // warpgroups whose P is outstanding
   uint32_t sw = 0, rest_s = 0, pw = 0, rest_p = 0;               // words of the chunks at hand, warpgroups left of them
-  uint32_t ks = 0, kph = 0, vs = 0, vph = 0, nq = 0, np[2] = {0, 0};
+  uint32_t ks = 0, kph = 0, vs = 0, vph = 0, nq = 0, np0 = 0, np1 = 0;
   uint32_t cs = 0, cp = 0, scrubs = 0;                           // chunks begun by S / by PV, scrubbed ones passed
-  bool stop = false;
+  bool stop = false, v_there = false;
   uint64_t idle_since = 0;
   uint32_t spins = 0;
   while (true) {
     bool moved = false;
     if (rest_p == 0 && cp < cs) {
-      pw = S.word[cp++ % kRing];
+      pw = uniform(S.word[cp++ % kRing]);
       rest_p = pw & kGroups;
+      v_there = false;
     }
-    if (rest_p != 0) {
+    if (rest_p != 0 && !v_there && ready(&S.v_full[vs], vph) &&
+        (!(pw & kScrubbed) || ready(&S.v_ready[scrubs % kRing], (scrubs / kRing) & 1u))) {
+      v_there = true;
+      if (pw & kScrubbed) ++scrubs;
+    }
+    if (rest_p != 0 && v_there) {
       const uint32_t wg = (rest_p & 1u) ? 0u : 1u;
-      const bool opens = rest_p == (pw & kGroups);
-      if (((waiting >> wg) & 1u) && ready(&S.p_full[wg], np[wg] & 1u) &&
-          (!opens || (ready(&S.v_full[vs], vph) &&
-                      (!(pw & kScrubbed) || ready(&S.v_ready[scrubs % kRing], (scrubs / kRing) & 1u))))) {
+      if (((waiting >> wg) & 1u) && ready(&S.p_full[wg], (wg ? np1 : np0) & 1u)) {
         tc_fence_after();
-        ++np[wg];
-        if (opens && (pw & kScrubbed)) ++scrubs;
-        const uint32_t add = !((pw & kBegins) >> 2 >> wg & 1u) || *(volatile uint32_t*)&S.zeroed[wg] != 0;
-        const uint32_t pa = tmem + kColS + 128 * wg, d = tmem + 128 * wg;
-        const uint64_t vd = v0 + vs * v_step;
-        mma_bf16_ts(d, pa, vd, id_o, add);
+        np0 += wg ^ 1u;
+        np1 += wg;
+        const uint32_t add = !(((pw & kBegins) >> 2 >> wg) & 1u) ? 1u : uniform(*(volatile uint32_t*)&S.zeroed[wg]);
+        const uint32_t pa = tmem + kColS + 128 * wg, d = tmem + 128 * wg, vl = v0 + vs * v_step;
+        const bool frees = rest_p == (1u << wg), ends = ((pw & kEnds) >> 4 >> wg) & 1u;
+        if (elect()) {
+          mma_bf16_ts(d, pa, desc(hi_v, vl), id_o, add);
 #pragma unroll
-        for (int i = 1; i < kKeys / 16; ++i) mma_bf16_ts(d, pa + i * 8, vd + (uint32_t)(i * (2048 >> 4)), id_o, 1);
+          for (int i = 1; i < kKeys / 16; ++i) mma_bf16_ts(d, pa + i * 8, desc(hi_v, vl + i * (2048 >> 4)), id_o, 1);
+          if (frees) mma_commit(&S.v_empty[vs]);
+          if (ends) mma_commit(&S.pv_done[wg]);
+        }
+        __syncwarp();
         waiting &= ~(1u << wg);
         rest_p &= ~(1u << wg);
-        if (rest_p == 0) {
-          mma_commit(&S.v_empty[vs]);
-          if (++vs == (uint32_t)a.vst) {
-            vs = 0;
-            vph ^= 1u;
-          }
+        if (frees && ++vs == (uint32_t)a.vst) {
+          vs = 0;
+          vph ^= 1u;
         }
-        if (((pw & kEnds) >> 4 >> wg) & 1u) mma_commit(&S.pv_done[wg]);
         moved = true;
       }
     }
@@ -325,38 +346,36 @@ __device__ __forceinline__ void issue(const Args& a, Shared& S, uint8_t* sq, uin
         tc_fence_after();
         nq += opens ? 1u : 0u;
         const uint32_t d = tmem + kColS + 128 * wg;
-        uint64_t qx = q0 + (((sw & kRows) && wg) ? q_tile : 0u), kx = k0 + ks * k_step;
-        uint32_t add = 0;
-#pragma unroll 1
-        for (int x = a.nkq; x > 1; --x) {
-          mma_bf16_ss(d, qx, kx, id_s, add);
-          mma_bf16_ss(d, qx + 2, kx + 2, id_s, 1);
-          mma_bf16_ss(d, qx + 4, kx + 4, id_s, 1);
-          mma_bf16_ss(d, qx + 6, kx + 6, id_s, 1);
-          qx += kQSlab >> 4;
-          kx += kSlab >> 4;
-          add = 1;
+        const uint32_t qx = q0 + (((sw & kRows) && wg) ? q_tile : 0u), kx = k0 + ks * k_step;
+        const bool frees = rest_s == (1u << wg);
+        if (elect()) {
+#pragma unroll
+          for (int x = 0; x < 3; ++x) {                          // d_qk up to 192 fits this kernel's shared memory
+            if (x < a.nkq) {
+              const uint32_t qy = qx + x * (kQSlab >> 4), ky = kx + x * (kSlab >> 4);
+              const int steps = x + 1 < a.nkq ? 4 : tail;
+              mma_bf16_ss(d, desc(hi_k, qy), desc(hi_k, ky), id_s, x != 0);
+              if (steps > 1) mma_bf16_ss(d, desc(hi_k, qy + 2), desc(hi_k, ky + 2), id_s, 1);
+              if (steps > 2) mma_bf16_ss(d, desc(hi_k, qy + 4), desc(hi_k, ky + 4), id_s, 1);
+              if (steps > 3) mma_bf16_ss(d, desc(hi_k, qy + 6), desc(hi_k, ky + 6), id_s, 1);
+            }
+          }
+          mma_commit(&S.s_full[wg]);
+          if (frees) mma_commit(&S.k_empty[ks]);
+          if (frees && (sw & kCloses)) mma_commit(&S.q_empty);
         }
-        mma_bf16_ss(d, qx, kx, id_s, add);
-        if (tail > 1) mma_bf16_ss(d, qx + 2, kx + 2, id_s, 1);
-        if (tail > 2) mma_bf16_ss(d, qx + 4, kx + 4, id_s, 1);
-        if (tail > 3) mma_bf16_ss(d, qx + 6, kx + 6, id_s, 1);
-        mma_commit(&S.s_full[wg]);
+        __syncwarp();
         waiting |= 1u << wg;
         rest_s &= ~(1u << wg);
-        if (rest_s == 0) {
-          mma_commit(&S.k_empty[ks]);
-          if (++ks == (uint32_t)a.kst) {
-            ks = 0;
-            kph ^= 1u;
-          }
-          if (sw & kCloses) mma_commit(&S.q_empty);
+        if (frees && ++ks == (uint32_t)a.kst) {
+          ks = 0;
+          kph ^= 1u;
         }
         moved = true;
       }
     }
     if (!stop && rest_s == 0 && ready(&S.k_full[ks], kph)) {
-      sw = S.word[cs % kRing];
+      sw = uniform(S.word[cs % kRing]);
       stop = (sw & kStop) != 0;
       rest_s = stop ? 0u : sw & kGroups;
       cs += stop ? 0u : 1u;
@@ -368,7 +387,7 @@ __device__ __forceinline__ void issue(const Args& a, Shared& S, uint8_t* sq, uin
     }
     if (stop && rest_p == 0 && cp == cs) return;
     if ((++spins & 63) != 0) continue;
-    const uint64_t now = global_timer_ns();
+    const uint64_t now = __shfl_sync(0xffffffffu, global_timer_ns(), 0);
     if (idle_since == 0) {
       idle_since = now;
     } else if (now - idle_since > kWaitLimitNs) {
@@ -432,6 +451,7 @@ __device__ __forceinline__ void scale_packed<__half>(float& word, float f) {
 // O (o_cols columns) and P (p_cols columns of packed pairs) times fac, in TMEM.
 template <typename T>
 __device__ __noinline__ void rescale(uint32_t to, int o_cols, uint32_t tp, int p_cols, float fac) {
+  tmem_st_wait();
 #pragma unroll 1
   for (int y = 0; y < o_cols; y += 16) {
     float o[16];
@@ -453,6 +473,56 @@ __device__ __noinline__ void rescale(uint32_t to, int o_cols, uint32_t tp, int p
   tmem_st_wait();
 }
 
+// Non-finite elements that the scrub took out of V (rows `bad` of the 32 keys from k0 on), added to the
+// query row if it sees them; `zero`: O holds nothing yet.
+template <typename T>
+__device__ __noinline__ void add_nonfinite(const Args& a, const Piece& g, int k0, uint32_t to, bool zero, uint32_t bad,
+                                           uint32_t vis) {
+  const SfaTreeParams& p = a.p;
+  if (zero) {
+    const float z[16] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int y = 0; y < a.dvp; y += 16) tmem_st16(to + y, z);
+    tmem_st_wait();
+  }
+#pragma unroll 1
+  for (; bad; bad &= bad - 1) {
+    const int b = __ffs(bad) - 1;
+    const bool sees = (vis >> b) & 1u;
+    const int row = box_row(p, g, k0 + b);
+    const T* v = static_cast<const T*>(p.v) + (int64_t)max(row, 0) * p.v_st + (int64_t)g.h * p.v_sh;
+#pragma unroll 1
+    for (int y = 0; y < a.dvp; y += 16) {
+      float o[16];
+      tmem_ld16(to + y, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = sees && y + i < p.d_v ? as_f(v[y + i]) : 0.f;
+        if (!isfinite(e)) o[i] += e;
+      }
+      tmem_st16(to + y, o);
+    }
+    tmem_st_wait();
+  }
+}
+
+// P of 32 keys, exp2(s c2 - m) with m in nm2's lanes negated, packed into 16 columns; their sum into `sum`.
+template <typename T>
+__device__ __forceinline__ void exps(const float (&s)[32], uint64_t c22, uint64_t nm2, uint64_t& sum, uint32_t tp) {
+  float pk[16];
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) {
+    float p0, p1;
+    untwo(fma2(two(s[k], s[k + 1]), c22, nm2), p0, p1);
+    p0 = ex2(p0);
+    p1 = ex2(p1);
+    sum = add2(sum, two(p0, p1));
+    pk[k / 2] = __uint_as_float(pack2<T>(p0, p1));
+  }
+  tmem_st16(tp, pk);
+}
+
 template <typename T>
 __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32_t tmem) {
   const SfaTreeParams& p = a.p;
@@ -461,6 +531,7 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
   const float c2 = p.scale * kLog2e;
   const uint64_t c22 = two(c2, c2);
   const bool by_tree = p.parents != nullptr;
+  const int my_node = a.n_hg > 1 ? 0 : m / a.GB, m_head = m - my_node * a.GB;
   Walk walk(a, S.range);
   Piece g;
   int n = 0, jobs = 0, met = 0, joined = 0, base = 0, scrubs = 0;   // tasks, ended pieces, meetings, joins; chunks and scrubs before the job
@@ -473,17 +544,17 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
     const Job j = make_job(a, g);
     const int tile = (a.two ? 2 * blockIdx.y : blockIdx.y) + (j.rows ? wg : 0);
     const int node0 = node_of_tile(a, tile);
-    const int my_node = a.n_hg > 1 ? 0 : m / a.GB;
-    const int my_head = a.n_hg > 1 ? (tile % a.n_hg) * 128 + m : m % a.GB;
+    const int my_head = a.n_hg > 1 ? (tile % a.n_hg) * 128 + m : m_head;
     const int node = node0 + my_node;
     const bool live = my_node < a.NT && my_head < a.G && node < g.q.rows && g.q.q0 + node < p.total_q;
     const bool any = __any_sync(0xffffffffu, live);
-    const int prefix = g.q.prefix;
+    const int prefix = g.q.prefix, rows_of = g.q.rows, job_c0 = j.c0, job_scrub = j.scrub;
     const int c_first = j.rows ? j.c0 : j.c0 + wg, c_end = j.rows ? (wg ? j.end_b : j.end_a) : j.end, c_step = j.rows ? 1 : 2;
     const bool ran = c_first < c_end;
-    if (by_tree && ran && c_end * kKeys > prefix) {
+    const bool tree = by_tree && g.q.rows > 1;                // a lone row sees the same either way
+    if (tree && ran && c_end * kKeys > prefix) {
+      // every warp has read the ancestors of the piece before (it waited for that piece's last PV)
       const int rows = min(g.q.rows, min(kMaxNodes, p.total_q - g.q.q0));
-      if (!(ok = meet(11))) break;                            // the piece before is done with both
 #pragma unroll 1
       for (int i = m; i < rows; i += 128) S.parent[wg][i] = (short)max(-1, min(__ldg(p.parents + g.q.q0 + i), i));
       if (!(ok = meet(12))) break;
@@ -492,7 +563,7 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
     }
     float mref = -INFINITY, l = 0.f;
     for (int c = c_first; c < c_end; c += c_step, ++n) {
-      const int cn = base + (c - j.c0);
+      const int cn = base + (c - job_c0);
       const bool first = c == c_first;
       if (!(ok = wtw(&S.s_full[wg], n & 1, a.status, 14))) break;
       tc_fence_after();
@@ -505,71 +576,58 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
       if (any) {
         if (drafted) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vis[i] &= sees32(S.anc[wg][my_node], by_tree, node, d0 + 32 * i);
+          for (int i = 0; i < 4; ++i) vis[i] &= sees32(S.anc[wg][my_node], tree, node, d0 + 32 * i);
         }
-        uint64_t sum0 = 0, sum1 = 0;
-        // 64 keys at a time in a loop that is not unrolled: with the 128 keys unrolled the softmax, issue
-        // and producer loops together miss the instruction cache on every pass (a third of all stalls:
-        // 515 us against 323 for 8 trees of 64 nodes at 32 keys a pass)
+        // 64 keys at a time in a loop that is not unrolled, for the sake of the instruction cache
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
-          float s[2][32];
-          ld32(ts + 64 * i, s[0]);
-          ld32(ts + 64 * i + 32, s[1]);
-          ld_wait32(s[0]);
-          ld_wait32(s[1]);
+          // loaded and waited for in one place: a load in flight across a call (a slow wait, a rescale)
+          // would land in registers that the call has saved or given away
+          float s0[32], s1[32];
+          ld32(ts + 64 * i, s0);
+          ld32(ts + 64 * i + 32, s1);
+          ld_wait32(s0);
+          ld_wait32(s1);
           if (!whole) {
             const uint32_t v0 = !live ? 0u : i ? vis[2] : vis[0], v1 = !live ? 0u : i ? vis[3] : vis[1];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-              if (!((v0 >> k) & 1u)) s[0][k] = -INFINITY;
-              if (!((v1 >> k) & 1u)) s[1][k] = -INFINITY;
+              if (!((v0 >> k) & 1u)) s0[k] = -INFINITY;
+              if (!((v1 >> k) & 1u)) s1[k] = -INFINITY;
             }
           }
-          float x[8];
+          // P against the reference maximum so far.  The maximum of these keys is not needed for that: if
+          // their sum stays below kMost, so does every P (and an infinite or a first one does not), and
+          // only otherwise is the reference raised and P done again.
+          float part;
+          for (bool again = false;; again = true) {
+            const float nm = mref == -INFINITY ? 0.f : -mref;
+            const uint64_t nm2 = two(nm, nm);
+            uint64_t sum0 = 0, sum1 = 0;
+            exps<T>(s0, c22, nm2, sum0, ts + 32 * i);         // over columns of S that have been read
+            exps<T>(s1, c22, nm2, sum1, ts + 32 * i + 16);
+            float t0, t1;
+            untwo(add2(sum0, sum1), t0, t1);
+            part = t0 + t1;
+            const bool up = live && (part > kMost || mref == -INFINITY);
+            if (again || !__any_sync(0xffffffffu, up)) break;
+            float top = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = fmaxf(s[0][k], s[1][k]);
-#pragma unroll
-          for (int k = 8; k < 32; ++k) x[k & 7] = fmaxf(x[k & 7], fmaxf(s[0][k], s[1][k]));
-          const float top =
-              fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * c2;
-          const bool up = live && (top > mref + kRescaleLog2 || (mref == -INFINITY && top > -INFINITY));
-          if (__any_sync(0xffffffffu, up)) {
+            for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaxf(s0[k], s1[k]));
+            top *= c2;
             float fac = 1.f;
-            if (up) {
+            if (up && top > mref) {
               if (mref != -INFINITY) fac = ex2(mref - top);
               mref = top;
             }
             if (__any_sync(0xffffffffu, fac != 1.f)) {
-              // rare: O, the sums and this chunk's P so far to the raised maximum
-              const uint64_t f2 = two(fac, fac);
-              sum0 = fma2(sum0, f2, 0ull);
-              sum1 = fma2(sum1, f2, 0ull);
+              // O, the sum and P of the chunk's first half to the raised maximum
               l *= fac;
               rescale<T>(to, first ? 0 : a.dvp, ts, 32 * i, fac);
             }
           }
-          const float nm = mref == -INFINITY ? 0.f : -mref;   // nothing seen yet: any reference gives p = 0
-          const uint64_t nm2 = two(nm, nm);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float pk[16];
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float p0, p1;
-              untwo(fma2(two(s[h][k], s[h][k + 1]), c22, nm2), p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-              if (k & 2) sum1 = add2(sum1, two(p0, p1));
-              else sum0 = add2(sum0, two(p0, p1));
-              pk[k / 2] = __uint_as_float(pack2<T>(p0, p1));
-            }
-            tmem_st16(ts + 32 * i + 16 * h, pk);              // over columns of S that have been read
-          }
+          l += part;                                          // zero where no key is seen
         }
-        float s0, s1;
-        untwo(add2(sum0, sum1), s0, s1);
-        l += s0 + s1;
         tmem_st_wait();
       }
       if (first) {
@@ -579,41 +637,18 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
           owe = false;
         }
       }
-      if (drafted && g.q.rows > 1) {
-        const int k = scrubs + (c - j.scrub);
+      if (drafted && rows_of > 1) {
+        const int k = scrubs + (c - job_scrub);
         if (!(ok = wtw(&S.v_ready[k % kRing], (k / kRing) & 1, a.status, 16))) break;
-        const uint32_t* bad = S.bad[k % kRing];
-        if (bad[0] | bad[1] | bad[2] | bad[3]) {
-          // non-finite elements that the scrub took out of V, for the rows that see them
+        const uint4 bad = *reinterpret_cast<const uint4*>(S.bad[k % kRing]);
+        if (bad.x | bad.y | bad.z | bad.w) {
           tc_fence_after();
-          if (first) {
-            const float z[16] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-            for (int y = 0; y < a.dvp; y += 16) tmem_st16(to + y, z);
-            tmem_st_wait();
-            if (m == 0) S.zeroed[wg] = 1;
-          }
-#pragma unroll 1
-          for (int b = 0; b < kKeys; ++b) {
-            if (!((bad[b >> 5] >> (b & 31)) & 1u)) continue;
-            const uint32_t mine = b < 32 ? vis[0] : b < 64 ? vis[1] : b < 96 ? vis[2] : vis[3];
-            const bool sees = live && ((mine >> (b & 31)) & 1u);
-            const int row = box_row(p, g, c * kKeys + b);
-            const T* v = static_cast<const T*>(p.v) + (int64_t)max(row, 0) * p.v_st + (int64_t)g.h * p.v_sh;
-#pragma unroll 1
-            for (int y = 0; y < a.dvp; y += 16) {
-              float o[16];
-              tmem_ld16(to + y, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float e = sees && y + i < p.d_v ? as_f(v[y + i]) : 0.f;
-                if (!isfinite(e)) o[i] += e;
-              }
-              tmem_st16(to + y, o);
-            }
-            tmem_st_wait();
-          }
+          const bool mine = live && any;
+          add_nonfinite<T>(a, g, c * kKeys, to, first, bad.x, mine ? vis[0] : 0u);
+          add_nonfinite<T>(a, g, c * kKeys + 32, to, false, bad.y, mine ? vis[1] : 0u);
+          add_nonfinite<T>(a, g, c * kKeys + 64, to, false, bad.z, mine ? vis[2] : 0u);
+          add_nonfinite<T>(a, g, c * kKeys + 96, to, false, bad.w, mine ? vis[3] : 0u);
+          if (first && m == 0) S.zeroed[wg] = 1;
         }
       }
       tc_fence_before();
@@ -674,24 +709,23 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
       }
 #pragma unroll 1
       for (int y = 0; y < a.dvp; y += 16) {
-        float o[16];
-        if (ran) {
+        float o[16] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (ran) {                                            // warp-uniform: the TMEM loads are the whole warp's
           tmem_ld16(to + y, o);
           tmem_ld_wait();
-        }
-        if (join) {
-          float ob[16];
-          tmem_ld16(tl + 128 + y, ob);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = (fa == 0.f ? 0.f : o[i] * fa) + (fb == 0.f ? 0.f : ob[i] * fb);
-        } else if (ran) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] *= fa;
-        }
-        if (none || !ran) {
+          if (join) {
+            float ob[16];
+            tmem_ld16(tl + 128 + y, ob);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0.f;
+            for (int i = 0; i < 16; ++i) o[i] = fmaf(ob[i], fb, o[i]);
+          }
+          if (none) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = 0.f;
+          }
         }
         if (live) {
           if (split) {
@@ -761,7 +795,7 @@ tree_pair_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtenso
   if (warp < 2) {
     produce(a, S, warp == 0, warp == 0 ? sk : sv, sq, warp == 0 ? &tmk : &tmv, &tmq);
   } else if (warp == 2) {
-    if ((threadIdx.x & 31) == 0) issue(a, S, sq, sk, sv, tmem, type_bits<T>());
+    issue(a, S, sq, sk, sv, tmem, type_bits<T>());
   } else if (warp == 3) {
     scrub<T>(a, S, sv);
   } else {
