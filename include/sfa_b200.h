@@ -304,7 +304,8 @@ int sfa_indexer_topk(const SfaIndexerParams* p, void* workspace, size_t workspac
  * rounded once to the tensor's type.  Pair i is (i, i + rot/2) of the rotated
  * part, or (2i, 2i + 1) when interleaved.  Angles are reduced exactly: the
  * position multiplies the frequency as a 64-bit fraction of a turn, so far
- * positions keep full accuracy.
+ * positions keep full accuracy.  dim is at most 1024, and a tensor has fewer than
+ * 2^31 rows.
  *
  * Up to three tensors go through one launch (q, k and, for the append, v with
  * neither weight nor TURN).  A tensor with SFA_ROTARY_PAGED is stored into a

@@ -10,10 +10,12 @@
 // any size keep the accuracy of sincospif.
 //
 // Memory-bound: every row is read once and written once, in fp32 registers
-// between.  A row is spread over L lanes (8 elements each: four of the lower
-// and four of the upper half of the rotated part, so that both members of a
-// pair are in one lane); 32/L rows of one token go through a warp at a time and
-// share the token's cosines, several of them in flight.
+// between.  A row is spread over L lanes, each with two runs of P elements, so
+// that both members of its P pairs are in the lane (half layout: P of the lower
+// and P of the upper half; interleaved: 2P neighbours).  P = 8 where 16-byte
+// accesses allow it, else 4.  32/L rows of one token go through a warp at a time;
+// the token's cosines and sines are computed once, a pair per lane, and handed
+// around in shared memory.  Arithmetic is on pairs of fp32 (f32x2).
 #include "sfa_common.cuh"
 #include "sfa_internal.h"
 
@@ -25,46 +27,6 @@ namespace rotary {
 
 constexpr int kWarps = 8;
 constexpr int kMaxDim = 1024;
-
-// Four consecutive elements as fp32.
-template <typename T>
-struct Quad;
-template <>
-struct Quad<float> {
-  float4 r;
-  __device__ __forceinline__ void load(const float* p) { r = __ldg(reinterpret_cast<const float4*>(p)); }
-  __device__ __forceinline__ void get(float* v) const { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-  static __device__ __forceinline__ void store(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-template <>
-struct Quad<__nv_bfloat16> {
-  uint2 r;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldg(reinterpret_cast<const uint2*>(p)); }
-  __device__ __forceinline__ void get(float* v) const {
-    v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
-    v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* v) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2_rn(v[0], v[1]), pack_bf16x2_rn(v[2], v[3]));
-  }
-};
-template <>
-struct Quad<__half> {
-  uint2 r;
-  __device__ __forceinline__ void load(const __half* p) { r = __ldg(reinterpret_cast<const uint2*>(p)); }
-  __device__ __forceinline__ void get(float* v) const {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-  }
-  static __device__ __forceinline__ void store(__half* p, const float* v) {
-    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  }
-};
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -108,6 +70,7 @@ __device__ __forceinline__ int64_t pool_row(const SfaRotaryParams& p, int t) {
     // last sequence that starts at or before t: 32 bounds at a time
     const int lane = threadIdx.x & 31;
     int lo = 0, span = p.num_seqs;
+#pragma unroll 1
     while (span > 1) {
       const int step = (span + 31) >> 5, at = lo + lane * step;
       const bool in = lane * step < span && __ldg(p.cu_seqlens + at) <= t;
@@ -132,33 +95,111 @@ __device__ __forceinline__ int64_t pool_row(const SfaRotaryParams& p, int t) {
   return (int64_t)pg * p.page_size + at % p.page_size;
 }
 
-// The eight elements (lo .. lo+3, hi .. hi+3) of unit u and its first pair (-1: not turned).
-struct Unit {
-  int lo, hi, pair;
-};
-__device__ __forceinline__ Unit unit_of(const SfaRotaryParams& p, bool turned, int u) {
-  const int first = p.start >> 3, n = p.rot >> 3;
-  Unit r{8 * u, 8 * u + 4, -1};
-  if (turned && u >= first && u < first + n) {
-    r.pair = 4 * (u - first);
-    if (!p.interleaved) {
-      r.lo = p.start + r.pair;
-      r.hi = r.lo + (p.rot >> 1);
-    }
-  }
+// Two fp32 lanes in one register pair.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float2 untwo(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
-// Turn the unit's four pairs by (c, sgn * s).
-__device__ __forceinline__ void turn_unit(float (&v)[8], const float (&c)[4], const float (&s)[4], float sgn,
-                                          bool interleaved) {
+// P consecutive elements, as they lie in memory.
+template <typename T, int P>
+struct Run {
+  static constexpr int W = P * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if (W == 4) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = v.x; w[1] = v.y; w[W - 2] = v.z; w[W - 1] = v.w;
+    } else {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if (W == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[W - 2], w[W - 1]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+};
+
+template <typename T> __device__ __forceinline__ uint64_t widen(uint32_t w);
+template <> __device__ __forceinline__ uint64_t widen<__nv_bfloat16>(uint32_t w) {
+  return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ uint64_t widen<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return two(f.x, f.y);
+}
+template <typename T> __device__ __forceinline__ uint32_t narrow(uint64_t v);
+template <> __device__ __forceinline__ uint32_t narrow<__nv_bfloat16>(uint64_t v) {
+  const float2 f = untwo(v);
+  return pack_bf16x2_rn(f.x, f.y);
+}
+template <> __device__ __forceinline__ uint32_t narrow<__half>(uint64_t v) {
+  const float2 f = untwo(v);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The lane's pairs as (first members, second members), two pairs to a register pair: j holds pairs
+// (2j, 2j+1) of the lane in the half layout and (j, j + P/2) interleaved, where it swaps the words'
+// halves (its own inverse).
+template <typename T, int P>
+__device__ __forceinline__ void take(const Run<T, P>& lo, const Run<T, P>& hi, bool inter, uint64_t (&a)[P / 2],
+                                     uint64_t (&b)[P / 2]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float sn = sgn * s[i];
-    const float a = interleaved ? v[2 * i] : v[i], b = interleaved ? v[2 * i + 1] : v[i + 4];
-    const float x = a * c[i] - b * sn, y = b * c[i] + a * sn;
-    if (interleaved) { v[2 * i] = x; v[2 * i + 1] = y; }
-    else { v[i] = x; v[i + 4] = y; }
+    for (int j = 0; j < P / 2; ++j) {
+      const float x0 = __uint_as_float(lo.w[2 * j]), x1 = __uint_as_float(lo.w[2 * j + 1]);
+      const float y0 = __uint_as_float(hi.w[2 * j]), y1 = __uint_as_float(hi.w[2 * j + 1]);
+      a[j] = inter ? two(x0, y0) : two(x0, x1);
+      b[j] = inter ? two(x1, y1) : two(y0, y1);
+    }
+  } else {
+    const uint32_t sa = inter ? 0x5410u : 0x3210u, sb = inter ? 0x7632u : 0x7654u;
+#pragma unroll
+    for (int j = 0; j < P / 2; ++j) {
+      a[j] = widen<T>(__byte_perm(lo.w[j], hi.w[j], sa));
+      b[j] = widen<T>(__byte_perm(lo.w[j], hi.w[j], sb));
+    }
+  }
+}
+template <typename T, int P>
+__device__ __forceinline__ void give(const uint64_t (&a)[P / 2], const uint64_t (&b)[P / 2], bool inter, Run<T, P>& lo,
+                                     Run<T, P>& hi) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < P / 2; ++j) {
+      const float2 x = untwo(a[j]), y = untwo(b[j]);
+      lo.w[2 * j] = __float_as_uint(x.x);
+      lo.w[2 * j + 1] = __float_as_uint(inter ? y.x : x.y);
+      hi.w[2 * j] = __float_as_uint(inter ? x.y : y.x);
+      hi.w[2 * j + 1] = __float_as_uint(y.y);
+    }
+  } else {
+    const uint32_t sa = inter ? 0x5410u : 0x3210u, sb = inter ? 0x7632u : 0x7654u;
+#pragma unroll
+    for (int j = 0; j < P / 2; ++j) {
+      const uint32_t x = narrow<T>(a[j]), y = narrow<T>(b[j]);
+      lo.w[j] = __byte_perm(x, y, sa);
+      hi.w[j] = __byte_perm(x, y, sb);
+    }
   }
 }
 
@@ -169,50 +210,79 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// L lanes per row, NS units of eight elements per lane (unit s * L + lane).
-template <typename T, int L, int NS, bool BWD>
-__global__ void __launch_bounds__(kWarps * 32)
+// Row elements of a lane's unit: runs of P at lo and hi; the unit's first pair, -1 if it is not turned.
+struct Unit {
+  int lo, hi, pair;
+};
+template <int P>
+__device__ __forceinline__ Unit unit_of(const SfaRotaryParams& p, bool turned, int u) {
+  const int first = p.start / (2 * P), n = p.rot / (2 * P);
+  Unit r{2 * P * u, 2 * P * u + P, -1};
+  if (turned && u >= first && u < first + n) {
+    r.pair = P * (u - first);
+    if (!p.interleaved) {
+      r.lo = p.start + r.pair;
+      r.hi = r.lo + (p.rot >> 1);
+    }
+  }
+  return r;
+}
+
+// L lanes per row, NS units per lane (unit s * L + lane).  Dynamic shared memory: the turn steps of the
+// rot / 2 pairs, then their (cos, sin) for each warp's token.
+template <typename T, int P, int L, int NS, bool BWD>
+__global__ void __launch_bounds__(kWarps * 32, 2)
 rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__ Grid g) {
-  constexpr int RPW = 32 / L;
-  constexpr int U = NS == 1 ? (sizeof(T) == 2 ? 4 : 2) : 1;   // rows of a lane in flight
+  constexpr int RPW = 32 / L, H = P / 2;
+  constexpr int U = NS == 1 && !(BWD && P == 8) ? 2 : 1;       // rows of a lane in flight: 64 bytes at P = 8
+  extern __shared__ uint64_t steps[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = lane % L, sub = lane / L;
+  const int col = lane % L, sub = lane / L, pairs = p.rot >> 1;
+  float2* cs = reinterpret_cast<float2*>(steps + pairs) + warp * pairs;
   int ti = 0, cta = blockIdx.x;
   while (cta >= g.ctas[ti]) cta -= g.ctas[ti++];
   const SfaRotaryTensor& t = p.t[ti];
-  const bool turned = (t.flags & SFA_ROTARY_TURN) && p.rot > 0;
+  const bool turned = (t.flags & SFA_ROTARY_TURN) && p.rot > 0, inter = p.interleaved != 0;
   const bool norm = t.weight != nullptr;
   const bool paged = !BWD && (t.flags & SFA_ROTARY_PAGED);
-  const int units = p.dim >> 3;
+  const int units = p.dim / (2 * P);
 
+  if (turned) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < pairs; i += kWarps * 32) steps[i] = turn_step(__ldg(p.frequencies + i));
+    __syncthreads();
+  }
   Unit un[NS];
   bool has[NS];
-  float w[NS][8], acc[NS][8];
-  uint64_t step[NS][4];
+  uint64_t wa[NS][H], wb[NS][H], da[NS][H], db[NS][H];         // weights and their gradients, as take() orders pairs
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     const int u = s * L + col;
     has[s] = u < units;
-    un[s] = unit_of(p, turned, has[s] ? u : 0);
-    if (!has[s]) un[s].pair = -1;
+    un[s] = unit_of<P>(p, turned, has[s] ? u : 0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      acc[s][i] = 0.f;
-      w[s][i] = norm ? __ldg(t.weight + (i < 4 ? un[s].lo + i : un[s].hi + i - 4)) : 1.f;
+    for (int j = 0; j < H; ++j) {
+      // the elements of the two pairs of register j
+      const int a0 = un[s].lo + 2 * j, b0 = inter ? un[s].lo + 2 * j + 1 : un[s].hi + 2 * j;
+      const int a1 = inter ? un[s].hi + 2 * j : un[s].lo + 2 * j + 1, b1 = un[s].hi + 2 * j + 1;
+      da[s][j] = db[s][j] = 0;
+      wa[s][j] = norm ? two(__ldg(t.weight + a0), __ldg(t.weight + a1)) : two(1.f, 1.f);
+      wb[s][j] = norm ? two(__ldg(t.weight + b0), __ldg(t.weight + b1)) : two(1.f, 1.f);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) step[s][i] = un[s].pair >= 0 ? turn_step(__ldg(p.frequencies + un[s].pair + i)) : 0;
   }
 
   const float inv_dim = 1.f / (float)p.dim;
-  const int64_t items = (int64_t)p.batch * p.len * g.chunks[ti];
-  const int64_t stride = (int64_t)g.ctas[ti] * kWarps;
-  for (int64_t item = (int64_t)cta * kWarps + warp; item < items; item += stride) {
-    const int64_t tok = item / g.chunks[ti];
+  const uint32_t items = (uint32_t)(p.batch * p.len) * g.chunks[ti], stride = g.ctas[ti] * kWarps;
+#pragma unroll 1
+  for (uint32_t item = cta * kWarps + warp; item < items; item += stride) {
+    const uint32_t tok = item / (uint32_t)g.chunks[ti];
     const int h0 = (int)(item - tok * g.chunks[ti]) * g.heads_per[ti];
     const int h1 = min(h0 + g.heads_per[ti], t.heads);
-    const int b = (int)(tok / p.len), tt = (int)(tok - (int64_t)b * p.len);
+    const int b = p.batch == 1 ? 0 : (int)(tok / (uint32_t)p.len), tt = (int)tok - b * p.len;
     const T* x = static_cast<const T*>(t.x) + b * t.x_sb + tt * t.x_st;
+    const int64_t y_sh = BWD ? t.dx_sh : t.y_sh;
+    const T* dy = BWD ? static_cast<const T*>(t.dy) + b * t.dy_sb + tt * t.dy_st : nullptr;
+    const int64_t pos = turned ? position_of(p, b, tt) : 0;
     int64_t yo;
     bool stored = true;
     if (BWD) {
@@ -225,25 +295,37 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
       yo = b * t.y_sb + tt * t.y_st;
     }
     T* y = static_cast<T*>(BWD ? t.dx : t.y) + yo;
-    const T* dy = BWD ? static_cast<const T*>(t.dy) + b * t.dy_sb + tt * t.dy_st : nullptr;
-    const int64_t y_sh = BWD ? t.dx_sh : t.y_sh;
-    float c[NS][4], sn[NS][4];
-    const int64_t pos = turned ? position_of(p, b, tt) : 0;
+    if (turned) {
+      __syncwarp();
+#pragma unroll 1
+      for (int i = lane; i < pairs; i += 32) {
+        float c, s;
+        turn(steps[i], pos, p.amplitude, c, s);
+        cs[i] = make_float2(c, s);
+      }
+      __syncwarp();
+    }
+    uint64_t c[NS][H], sn[NS][H];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[s][i] = 1.f;
-        sn[s][i] = 0.f;
-        if (un[s].pair >= 0) turn(step[s][i], pos, p.amplitude, c[s][i], sn[s][i]);
+      for (int j = 0; j < H; ++j) {
+        c[s][j] = two(1.f, 1.f);
+        sn[s][j] = 0;
+        if (un[s].pair >= 0) {
+          const float2 u = cs[un[s].pair + (inter ? j : 2 * j)], v = cs[un[s].pair + (inter ? j + H : 2 * j + 1)];
+          c[s][j] = two(u.x, v.x);
+          sn[s][j] = two(u.y, v.y);
+        }
       }
+#pragma unroll 1
     for (int hb = h0; hb < h1; hb += RPW * U) {
-      Quad<T> xl[U][NS], xh[U][NS], gl[U][NS], gh[U][NS];
+      Run<T, P> xl[U][NS], xh[U][NS], gl[U][NS], gh[U][NS];
 #pragma unroll
       for (int r = 0; r < U; ++r) {
         const int h = hb + r * RPW + sub;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < NS; ++s)
           if (h < h1 && has[s]) {
             xl[r][s].load(x + h * t.x_sh + un[s].lo);
             xh[r][s].load(x + h * t.x_sh + un[s].hi);
@@ -252,62 +334,82 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
               gh[r][s].load(dy + h * t.dy_sh + un[s].hi);
             }
           }
-        }
       }
 #pragma unroll
       for (int r = 0; r < U; ++r) {
         const int h = hb + r * RPW + sub;
-        float v[NS][8], d[NS][8];
-        float sq = 0.f, sd = 0.f;
+        uint64_t va[NS][H], vb[NS][H], ga[NS][H], gb[NS][H];
+        uint64_t sq = 0, sd = 0;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           const bool on = h < h1 && has[s];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) { v[s][i] = 0.f; d[s][i] = 0.f; }
+          for (int j = 0; j < H; ++j) va[s][j] = vb[s][j] = ga[s][j] = gb[s][j] = 0;
           if (on) {
-            xl[r][s].get(v[s]);
-            xh[r][s].get(v[s] + 4);
+            take<T, P>(xl[r][s], xh[r][s], inter, va[s], vb[s]);
             if (BWD) {
-              gl[r][s].get(d[s]);
-              gh[r][s].get(d[s] + 4);
-              if (un[s].pair >= 0) turn_unit(d[s], c[s], sn[s], -1.f, p.interleaved);
+              take<T, P>(gl[r][s], gh[r][s], inter, ga[s], gb[s]);
+              if (un[s].pair >= 0) {
+#pragma unroll
+                for (int j = 0; j < H; ++j) {
+                  const uint64_t u = fma2(gb[s][j], sn[s][j], mul2(ga[s][j], c[s][j]));
+                  gb[s][j] = fma2(neg2(ga[s][j]), sn[s][j], mul2(gb[s][j], c[s][j]));
+                  ga[s][j] = u;
+                }
+              }
             }
           }
           if (norm) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              sq = fmaf(v[s][i], v[s][i], sq);
-              if (BWD) sd = fmaf(d[s][i] * w[s][i], v[s][i], sd);
+            for (int j = 0; j < H; ++j) {
+              sq = fma2(va[s][j], va[s][j], sq);
+              sq = fma2(vb[s][j], vb[s][j], sq);
+              if (BWD) {
+                sd = fma2(mul2(ga[s][j], wa[s][j]), va[s][j], sd);
+                sd = fma2(mul2(gb[s][j], wb[s][j]), vb[s][j], sd);
+              }
             }
           }
         }
         float rn = 1.f, k = 0.f;
         if (norm) {
-          sq = row_sum<L>(sq);
-          rn = rsqrtf(sq * inv_dim + p.eps);
-          if (BWD) k = row_sum<L>(sd) * inv_dim * rn * rn;
+          const float2 q2 = untwo(sq), d2 = untwo(sd);
+          rn = rsqrtf(row_sum<L>(q2.x + q2.y) * inv_dim + p.eps);
+          if (BWD) k = row_sum<L>(d2.x + d2.y) * inv_dim * rn * rn * rn;
         }
+        const uint64_t rn2 = two(rn, rn), k2 = two(-k, -k);
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           if (!(h < h1 && has[s])) continue;
-          float o[8];
+          uint64_t oa[H], ob[H];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (BWD) {
-              if (norm) {
-                acc[s][i] = fmaf(d[s][i], v[s][i] * rn, acc[s][i]);
-                o[i] = rn * (d[s][i] * w[s][i] - v[s][i] * k);
-              } else {
-                o[i] = d[s][i];
-              }
+          for (int j = 0; j < H; ++j) {
+            if (BWD && norm) {
+              da[s][j] = fma2(ga[s][j], mul2(va[s][j], rn2), da[s][j]);
+              db[s][j] = fma2(gb[s][j], mul2(vb[s][j], rn2), db[s][j]);
+              oa[j] = fma2(va[s][j], k2, mul2(mul2(ga[s][j], wa[s][j]), rn2));
+              ob[j] = fma2(vb[s][j], k2, mul2(mul2(gb[s][j], wb[s][j]), rn2));
+            } else if (BWD) {
+              oa[j] = ga[s][j];
+              ob[j] = gb[s][j];
             } else {
-              o[i] = v[s][i] * rn * w[s][i];
+              oa[j] = norm ? mul2(mul2(va[s][j], rn2), wa[s][j]) : va[s][j];
+              ob[j] = norm ? mul2(mul2(vb[s][j], rn2), wb[s][j]) : vb[s][j];
             }
           }
-          if (!BWD && un[s].pair >= 0) turn_unit(o, c[s], sn[s], 1.f, p.interleaved);
+          if (!BWD && un[s].pair >= 0) {
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              const uint64_t u = fma2(neg2(ob[j]), sn[s][j], mul2(oa[j], c[s][j]));
+              ob[j] = fma2(oa[j], sn[s][j], mul2(ob[j], c[s][j]));
+              oa[j] = u;
+            }
+          }
           if (stored) {
-            Quad<T>::store(y + h * y_sh + un[s].lo, o);
-            Quad<T>::store(y + h * y_sh + un[s].hi, o + 4);
+            Run<T, P> lo, hi;
+            give<T, P>(oa, ob, inter, lo, hi);
+            lo.store(y + h * y_sh + un[s].lo);
+            hi.store(y + h * y_sh + un[s].hi);
           }
         }
       }
@@ -316,21 +418,29 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
 
   if (BWD && t.dweight != nullptr) {
     // the CTA's sum of each column, rows in a fixed order
-    __shared__ float part[kWarps][NS * L * 8];
+    float* part = reinterpret_cast<float*>(steps);             // [kWarps][dim], over the turns
+    __syncthreads();
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v = acc[s][i];
+      for (int j = 0; j < H; ++j) {
+        const int a0 = un[s].lo + 2 * j, b0 = inter ? un[s].lo + 2 * j + 1 : un[s].hi + 2 * j;
+        const int a1 = inter ? un[s].hi + 2 * j : un[s].lo + 2 * j + 1, b1 = un[s].hi + 2 * j + 1;
+        const float2 va = untwo(da[s][j]), vb = untwo(db[s][j]);
+        float v[4] = {va.x, va.y, vb.x, vb.y};
+        const int at[4] = {a0, a1, b0, b1};
 #pragma unroll
-        for (int o = L; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (sub == 0 && has[s]) part[warp][i < 4 ? un[s].lo + i : un[s].hi + i - 4] = v;
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int o = L; o < 32; o <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+          if (sub == 0 && has[s]) part[warp * p.dim + at[i]] = v[i];
+        }
       }
     __syncthreads();
     for (int i = threadIdx.x; i < p.dim; i += kWarps * 32) {
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) v += part[k][i];
+      for (int w = 0; w < kWarps; ++w) v += part[w * p.dim + i];
       g.partial[(int64_t)blockIdx.x * p.dim + i] = v;
     }
   }
@@ -468,32 +578,43 @@ __global__ void rotary_dweight_kernel(const __grid_constant__ SfaRotaryParams p,
   }
 }
 
-static bool vector_ok(const SfaRotaryParams& p, bool bwd) {
-  if (p.dim % 8 || p.rot % 8 || p.start % 8) return false;
-  const uintptr_t bytes = p.dtype == SFA_DTYPE_F32 ? 16 : 8;   // four elements
-  auto ok = [&](const void* ptr, int64_t sb, int64_t st, int64_t sh) {
-    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && sb % 4 == 0 && st % 4 == 0 && sh % 4 == 0;
-  };
-  for (int i = 0; i < p.num_tensors; ++i) {
-    const SfaRotaryTensor& t = p.t[i];
-    if (!ok(t.x, t.x_sb, t.x_st, t.x_sh)) return false;
-    if (!bwd && !ok(t.y, t.y_sb, t.y_st, t.y_sh)) return false;
-    if (bwd && (!ok(t.dy, t.dy_sb, t.dy_st, t.dy_sh) || !ok(t.dx, t.dx_sb, t.dx_st, t.dx_sh))) return false;
-  }
-  return true;
-}
+// How a call runs: P elements a run (0: the kernel for any shape), L lanes a row, NS units a lane.
+struct Shape {
+  int p, lanes, units;
+};
 
-static int lanes_per_row(int dim) {
-  int l = 2;
-  while (l < 32 && l * 8 < dim) l *= 2;
-  return l;
+// The widest runs that sizes and alignment allow: every run of P elements starts at a multiple of P.
+static Shape shape_of(const SfaRotaryParams& p, bool bwd) {
+  const int size = p.dtype == SFA_DTYPE_F32 ? 4 : 2;
+  auto fits = [&](int n) {
+    if (p.dim % (2 * n) || p.rot % (2 * n) || p.start % (2 * n)) return false;
+    auto ok = [&](const void* ptr, int64_t sb, int64_t st, int64_t sh) {
+      return reinterpret_cast<uintptr_t>(ptr) % (n * size) == 0 && sb % n == 0 && st % n == 0 && sh % n == 0;
+    };
+    for (int i = 0; i < p.num_tensors; ++i) {
+      const SfaRotaryTensor& t = p.t[i];
+      if (!ok(t.x, t.x_sb, t.x_st, t.x_sh)) return false;
+      if (!bwd && !ok(t.y, t.y_sb, t.y_st, t.y_sh)) return false;
+      if (bwd && (!ok(t.dy, t.dy_sb, t.dy_st, t.dy_sh) || !ok(t.dx, t.dx_sb, t.dx_st, t.dx_sh))) return false;
+    }
+    return true;
+  };
+  Shape s{0, 32, 1};
+  if (size == 2 && fits(8)) s.p = 8;
+  else if (fits(4)) s.p = 4;
+  if (!s.p) return s;
+  const int units = p.dim / (2 * s.p);
+  s.lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32;
+  s.units = (units + 31) / 32;
+  if (s.p == 4 && s.units > 1) s.units = 4;        // P 4: up to 128 units
+  return s;
 }
 
 // Items of up to 32 warp steps share one token's cosines; fewer when there would
 // be too few items to fill the SMs (a decode step), down to one step each.
-static Grid make_grid(const SfaRotaryParams& p, bool vec) {
+static Grid make_grid(const SfaRotaryParams& p, const Shape& s) {
   Grid g{};
-  const int sms = device_sm_count(), rpw = vec ? 32 / lanes_per_row(p.dim) : 1;
+  const int sms = device_sm_count(), rpw = s.p ? 32 / s.lanes : 1;
   const int64_t tokens = (int64_t)p.batch * p.len;
   int64_t heads = 0;
   for (int i = 0; i < p.num_tensors; ++i) heads += p.t[i].heads;
@@ -501,7 +622,7 @@ static Grid make_grid(const SfaRotaryParams& p, bool vec) {
   const int per = (int)std::min<int64_t>(32, std::max<int64_t>(1, steps / ((int64_t)sms * 32)));
   const int most = sms * 8;
   for (int i = 0; i < p.num_tensors; ++i) {
-    g.heads_per[i] = vec ? std::min(p.t[i].heads, per * rpw) : 1;
+    g.heads_per[i] = s.p ? std::min(p.t[i].heads, per * rpw) : 1;
     g.chunks[i] = (p.t[i].heads + g.heads_per[i] - 1) / g.heads_per[i];
     const int64_t ctas = (tokens * g.chunks[i] + kWarps - 1) / kWarps;
     const int64_t share = std::max<int64_t>(1, most * (int64_t)p.t[i].heads / heads);
@@ -516,29 +637,38 @@ static int total_ctas(const SfaRotaryParams& p, const Grid& g) {
   return n;
 }
 
+template <typename T, int P, bool BWD>
+static void launch_runs(const SfaRotaryParams& p, const Grid& g, const Shape& s, cudaStream_t st) {
+  const int n = total_ctas(p, g), threads = kWarps * 32;
+  const size_t smem = std::max((size_t)(p.rot / 2) * (sizeof(uint64_t) + kWarps * sizeof(float2)),   // at most 36 KB
+                               BWD ? kWarps * sizeof(float) * p.dim : (size_t)0);
+  if (s.units == 1) {
+    if (s.lanes == 4) rotary_kernel<T, P, 4, 1, BWD><<<n, threads, smem, st>>>(p, g);
+    else if (s.lanes == 8) rotary_kernel<T, P, 8, 1, BWD><<<n, threads, smem, st>>>(p, g);
+    else if (s.lanes == 16) rotary_kernel<T, P, 16, 1, BWD><<<n, threads, smem, st>>>(p, g);
+    else rotary_kernel<T, P, 32, 1, BWD><<<n, threads, smem, st>>>(p, g);
+  } else {
+    rotary_kernel<T, P, 32, P == 8 ? 2 : 4, BWD><<<n, threads, smem, st>>>(p, g);   // above 512 (256) dims
+  }
+}
+
 template <typename T, bool BWD>
-static void launch_typed(const SfaRotaryParams& p, const Grid& g, bool vec, cudaStream_t st) {
-  const int n = total_ctas(p, g);
-  const int threads = kWarps * 32;
-  if (!vec) {
-    rotary_any_kernel<T, BWD><<<n, threads, BWD ? sizeof(float) * kWarps * p.dim : 0, st>>>(p, g);
+static void launch_typed(const SfaRotaryParams& p, const Grid& g, const Shape& s, cudaStream_t st) {
+  if (s.p == 0) {
+    rotary_any_kernel<T, BWD><<<total_ctas(p, g), kWarps * 32, BWD ? sizeof(float) * kWarps * p.dim : 0, st>>>(p, g);
     return;
   }
-  const int l = lanes_per_row(p.dim);
-  if (l == 2) rotary_kernel<T, 2, 1, BWD><<<n, threads, 0, st>>>(p, g);
-  else if (l == 4) rotary_kernel<T, 4, 1, BWD><<<n, threads, 0, st>>>(p, g);
-  else if (l == 8) rotary_kernel<T, 8, 1, BWD><<<n, threads, 0, st>>>(p, g);
-  else if (l == 16) rotary_kernel<T, 16, 1, BWD><<<n, threads, 0, st>>>(p, g);
-  else if (p.dim <= 256) rotary_kernel<T, 32, 1, BWD><<<n, threads, 0, st>>>(p, g);
-  else if (p.dim <= 512) rotary_kernel<T, 32, 2, BWD><<<n, threads, 0, st>>>(p, g);
-  else rotary_kernel<T, 32, 4, BWD><<<n, threads, 0, st>>>(p, g);
+  if constexpr (sizeof(T) == 2) {
+    if (s.p == 8) return launch_runs<T, 8, BWD>(p, g, s, st);
+  }
+  launch_runs<T, 4, BWD>(p, g, s, st);
 }
 
 template <bool BWD>
-static void launch(const SfaRotaryParams& p, const Grid& g, bool vec, cudaStream_t st) {
-  if (p.dtype == SFA_DTYPE_BF16) launch_typed<__nv_bfloat16, BWD>(p, g, vec, st);
-  else if (p.dtype == SFA_DTYPE_F16) launch_typed<__half, BWD>(p, g, vec, st);
-  else launch_typed<float, BWD>(p, g, vec, st);
+static void launch(const SfaRotaryParams& p, const Grid& g, const Shape& s, cudaStream_t st) {
+  if (p.dtype == SFA_DTYPE_BF16) launch_typed<__nv_bfloat16, BWD>(p, g, s, st);
+  else if (p.dtype == SFA_DTYPE_F16) launch_typed<__half, BWD>(p, g, s, st);
+  else launch_typed<float, BWD>(p, g, s, st);
 }
 
 static int bad(const std::string& m) { return report_error(SFA_ERR_INVALID_ARGUMENT, "rotary: " + m); }
@@ -555,6 +685,7 @@ static int check(const SfaRotaryParams* p, bool bwd) {
   for (int i = 0; i < p->num_tensors; ++i) {
     const SfaRotaryTensor& t = p->t[i];
     if (t.heads < 1) return bad("heads must be positive");
+    if (!empty && (int64_t)p->batch * p->len >= INT32_MAX / t.heads) return bad("a tensor must have fewer than 2^31 rows");
     const bool no_pool = (t.flags & SFA_ROTARY_PAGED) && p->num_pages == 0;
     if (!empty && (!t.x || (bwd ? !t.dy || !t.dx : !t.y && !no_pool))) return bad("tensor pointers must be non-NULL");
     if (!empty && (t.flags & SFA_ROTARY_TURN) && p->rot && (!p->positions || !p->frequencies))
@@ -583,9 +714,9 @@ int sfa_rotary_fwd(const SfaRotaryParams* p, void* stream) {
   const int rc = rotary::check(p, false);
   if (rc) return rc;
   if (p->batch == 0 || p->len == 0) return SFA_OK;
-  const bool vec = rotary::vector_ok(*p, false);
+  const rotary::Shape shape = rotary::shape_of(*p, false);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  rotary::launch<false>(*p, rotary::make_grid(*p, vec), vec, st);
+  rotary::launch<false>(*p, rotary::make_grid(*p, shape), shape, st);
   note_launch("rotary_fwd", st);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return report_error(SFA_ERR_CUDA, std::string("rotary forward: ") + cudaGetErrorString(e));
@@ -594,7 +725,7 @@ int sfa_rotary_fwd(const SfaRotaryParams* p, void* stream) {
 
 size_t sfa_rotary_bwd_workspace_bytes(const SfaRotaryParams* p) {
   if (rotary::check(p, true) || p->batch == 0 || p->len == 0) return 0;
-  const rotary::Grid g = rotary::make_grid(*p, rotary::vector_ok(*p, true));
+  const rotary::Grid g = rotary::make_grid(*p, rotary::shape_of(*p, true));
   return sizeof(float) * (size_t)rotary::total_ctas(*p, g) * p->dim;
 }
 
@@ -609,12 +740,12 @@ int sfa_rotary_bwd(const SfaRotaryParams* p, void* workspace, size_t workspace_b
     for (int i = 0; i < p->num_tensors && e == cudaSuccess; ++i)
       if (p->t[i].dweight) e = cudaMemsetAsync(p->t[i].dweight, 0, sizeof(float) * p->dim, st);
   } else {
-    const bool vec = rotary::vector_ok(*p, true);
-    rotary::Grid g = rotary::make_grid(*p, vec);
+    const rotary::Shape shape = rotary::shape_of(*p, true);
+    rotary::Grid g = rotary::make_grid(*p, shape);
     if (dw && (!workspace || workspace_bytes < sizeof(float) * (size_t)rotary::total_ctas(*p, g) * p->dim))
       return report_error(SFA_ERR_WORKSPACE, "rotary: workspace missing or too small");
     g.partial = static_cast<float*>(workspace);
-    rotary::launch<true>(*p, g, vec, st);
+    rotary::launch<true>(*p, g, shape, st);
     note_launch("rotary_bwd", st);
     e = cudaGetLastError();
     if (dw && e == cudaSuccess) {
