@@ -123,12 +123,12 @@ template <typename T, int P>
 struct Run {
   static constexpr int W = P * (int)sizeof(T) / 4;
   uint32_t w[W];
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void read(const uint8_t* p) {   // from shared memory
     if (W == 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
       w[0] = v.x; w[1] = v.y; w[W - 2] = v.z; w[W - 1] = v.w;
     } else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
       w[0] = v.x; w[1] = v.y;
     }
   }
@@ -137,6 +137,14 @@ struct Run {
     else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   }
 };
+
+// Asynchronous copy of N bytes (8 or 16) into shared memory.
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+}
 
 template <typename T> __device__ __forceinline__ uint64_t widen(uint32_t w);
 template <> __device__ __forceinline__ uint64_t widen<__nv_bfloat16>(uint32_t w) {
@@ -228,16 +236,55 @@ __device__ __forceinline__ Unit unit_of(const SfaRotaryParams& p, bool turned, i
   return r;
 }
 
-// L lanes per row, NS units per lane (unit s * L + lane).  Dynamic shared memory: the turn steps of the
-// rot / 2 pairs, then their (cos, sin) for each warp's token.
+// Steps of a warp whose rows are under way at a time.
+template <int NS>
+constexpr int stages() {
+  return NS == 1 ? 4 : 2;
+}
+// Bytes of the ring: every thread copies its own runs and reads them back, so it needs no barrier.
+template <typename T, int P, int NS, bool BWD>
+constexpr int ring_bytes() {
+  return stages<NS>() * NS * (BWD ? 4 : 2) * P * (int)sizeof(T) * kWarps * 32;
+}
+
+// The steps of a warp: 32 / L heads of a token at a time, item by item.
+struct Steps {
+  uint32_t item, items, stride;
+  int chunks, per, heads, b, tt, h, h1;
+  int len, batch;
+  __device__ __forceinline__ bool open() {
+    if (item >= items) return false;
+    const uint32_t tok = item / (uint32_t)chunks;
+    h = (int)(item - tok * chunks) * per;
+    h1 = min(h + per, heads);
+    b = batch == 1 ? 0 : (int)(tok / (uint32_t)len);
+    tt = (int)tok - b * len;
+    return true;
+  }
+  // to the next step; `fresh`: of another item
+  __device__ __forceinline__ bool next(int rpw, bool& fresh) {
+    h += rpw;
+    fresh = h >= h1;
+    if (!fresh) return true;
+    item += stride;
+    return open();
+  }
+};
+
+// L lanes per row, NS units per lane (unit s * L + lane).  The rows of the next steps are on their way
+// into shared memory while one is worked on.  Loaded into registers instead, a step's rows leave nothing
+// in flight while they are worked on: 763 us for norm, rotary and gradients of 4 x 8192 tokens of 64 + 4
+// heads of 128, against 538 us here.  Forward: 3 CTAs per SM (559 us with 2; the backward's registers allow 2).
+// Dynamic shared memory: the ring, the turn steps of the rot / 2 pairs, their (cos, sin) for each warp's token.
 template <typename T, int P, int L, int NS, bool BWD>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kWarps * 32, BWD || NS > 1 ? 2 : 3)
 rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__ Grid g) {
-  constexpr int RPW = 32 / L, H = P / 2;
-  constexpr int U = NS == 1 && !(BWD && P == 8) ? 2 : 1;       // rows of a lane in flight: 64 bytes at P = 8
-  extern __shared__ uint64_t steps[];
+  constexpr int RPW = 32 / L, H = P / 2, R = P * (int)sizeof(T), S = stages<NS>(), K = NS * (BWD ? 4 : 2);
+  extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = lane % L, sub = lane / L, pairs = p.rot >> 1;
+  uint8_t* ring = smem + threadIdx.x * R;                      // run k of stage s at (s * K + k) * kWarps * 32 * R
+  uint64_t* steps = reinterpret_cast<uint64_t*>(smem + ring_bytes<T, P, NS, BWD>());
   float2* cs = reinterpret_cast<float2*>(steps + pairs) + warp * pairs;
   int ti = 0, cta = blockIdx.x;
   while (cta >= g.ctas[ti]) cta -= g.ctas[ti++];
@@ -247,19 +294,58 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
   const bool paged = !BWD && (t.flags & SFA_ROTARY_PAGED);
   const int units = p.dim / (2 * P);
 
-  if (turned) {
-#pragma unroll 1
-    for (int i = threadIdx.x; i < pairs; i += kWarps * 32) steps[i] = turn_step(__ldg(p.frequencies + i));
-    __syncthreads();
-  }
   Unit un[NS];
   bool has[NS];
-  uint64_t wa[NS][H], wb[NS][H], da[NS][H], db[NS][H];         // weights and their gradients, as take() orders pairs
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     const int u = s * L + col;
     has[s] = u < units;
     un[s] = unit_of<P>(p, turned, has[s] ? u : 0);
+  }
+  Steps at;
+  at.items = (uint32_t)(p.batch * p.len) * g.chunks[ti];
+  at.item = cta * kWarps + warp;
+  at.stride = g.ctas[ti] * kWarps;
+  at.chunks = g.chunks[ti];
+  at.per = g.heads_per[ti];
+  at.heads = t.heads;
+  at.len = p.len;
+  at.batch = p.batch;
+  Steps ahead = at;
+  bool more = ahead.open(), fresh = true;
+  // asks for the rows of the step at `ahead`, into `stage`
+  auto ask = [&](int stage) {
+    if (more) {
+      const int h = ahead.h + sub;
+      const T* x = static_cast<const T*>(t.x) + ahead.b * t.x_sb + ahead.tt * t.x_st + h * t.x_sh;
+      const T* dy = BWD ? static_cast<const T*>(t.dy) + ahead.b * t.dy_sb + ahead.tt * t.dy_st + h * t.dy_sh : nullptr;
+      uint8_t* dst = ring + stage * K * kWarps * 32 * R;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        if (h < ahead.h1 && has[s]) {
+          copy_async<R>(dst + (s * (K / NS)) * kWarps * 32 * R, x + un[s].lo);
+          copy_async<R>(dst + (s * (K / NS) + 1) * kWarps * 32 * R, x + un[s].hi);
+          if (BWD) {
+            copy_async<R>(dst + (s * (K / NS) + 2) * kWarps * 32 * R, dy + un[s].lo);
+            copy_async<R>(dst + (s * (K / NS) + 3) * kWarps * 32 * R, dy + un[s].hi);
+          }
+        }
+      bool f;
+      more = ahead.next(RPW, f);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i < S - 1; ++i) ask(i);
+
+  if (turned) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < pairs; i += kWarps * 32) steps[i] = turn_step(__ldg(p.frequencies + i));
+    __syncthreads();
+  }
+  uint64_t wa[NS][H], wb[NS][H], da[NS][H], db[NS][H];         // weights and their gradients, as take() orders pairs
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int j = 0; j < H; ++j) {
       // the elements of the two pairs of register j
@@ -269,156 +355,149 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
       wa[s][j] = norm ? two(__ldg(t.weight + a0), __ldg(t.weight + a1)) : two(1.f, 1.f);
       wb[s][j] = norm ? two(__ldg(t.weight + b0), __ldg(t.weight + b1)) : two(1.f, 1.f);
     }
-  }
 
   const float inv_dim = 1.f / (float)p.dim;
-  const uint32_t items = (uint32_t)(p.batch * p.len) * g.chunks[ti], stride = g.ctas[ti] * kWarps;
+  const int64_t y_sh = BWD ? t.dx_sh : t.y_sh;
+  T* y = nullptr;
+  bool stored = true;
+  uint64_t c[NS][H], sn[NS][H];
+  int stage = 0;
+  bool have = at.open();
+  int64_t pos_next = have && turned ? position_of(p, at.b, at.tt) : 0;
 #pragma unroll 1
-  for (uint32_t item = cta * kWarps + warp; item < items; item += stride) {
-    const uint32_t tok = item / (uint32_t)g.chunks[ti];
-    const int h0 = (int)(item - tok * g.chunks[ti]) * g.heads_per[ti];
-    const int h1 = min(h0 + g.heads_per[ti], t.heads);
-    const int b = p.batch == 1 ? 0 : (int)(tok / (uint32_t)p.len), tt = (int)tok - b * p.len;
-    const T* x = static_cast<const T*>(t.x) + b * t.x_sb + tt * t.x_st;
-    const int64_t y_sh = BWD ? t.dx_sh : t.y_sh;
-    const T* dy = BWD ? static_cast<const T*>(t.dy) + b * t.dy_sb + tt * t.dy_st : nullptr;
-    const int64_t pos = turned ? position_of(p, b, tt) : 0;
-    int64_t yo;
-    bool stored = true;
-    if (BWD) {
-      yo = b * t.dx_sb + tt * t.dx_st;
-    } else if (paged) {
-      const int64_t row = pool_row(p, tt);
-      stored = row >= 0;
-      yo = stored ? row * t.y_st : 0;
-    } else {
-      yo = b * t.y_sb + tt * t.y_st;
-    }
-    T* y = static_cast<T*>(BWD ? t.dx : t.y) + yo;
-    if (turned) {
-      __syncwarp();
-#pragma unroll 1
-      for (int i = lane; i < pairs; i += 32) {
-        float c, s;
-        turn(steps[i], pos, p.amplitude, c, s);
-        cs[i] = make_float2(c, s);
+  while (have) {
+    if (fresh) {
+      const int b = at.b, tt = at.tt;
+      const int64_t pos = pos_next;
+      int64_t yo;
+      if (BWD) {
+        yo = b * t.dx_sb + tt * t.dx_st;
+      } else if (paged) {
+        const int64_t row = pool_row(p, tt);
+        stored = row >= 0;
+        yo = stored ? row * t.y_st : 0;
+      } else {
+        yo = b * t.y_sb + tt * t.y_st;
       }
-      __syncwarp();
-    }
-    uint64_t c[NS][H], sn[NS][H];
+      y = static_cast<T*>(BWD ? t.dx : t.y) + yo;
+      if (turned) {
+        __syncwarp();
+#pragma unroll 1
+        for (int i = lane; i < pairs; i += 32) {
+          float cc, ss;
+          turn(steps[i], pos, p.amplitude, cc, ss);
+          cs[i] = make_float2(cc, ss);
+        }
+        __syncwarp();
+        Steps then = at;                                       // the next item's position, on its way meanwhile
+        then.item += then.stride;
+        if (then.open()) pos_next = position_of(p, then.b, then.tt);
+      }
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          c[s][j] = two(1.f, 1.f);
+          sn[s][j] = 0;
+          if (un[s].pair >= 0) {
+            const float2 u = cs[un[s].pair + (inter ? j : 2 * j)], v = cs[un[s].pair + (inter ? j + H : 2 * j + 1)];
+            c[s][j] = two(u.x, v.x);
+            sn[s][j] = two(u.y, v.y);
+          }
+        }
+    }
+    const int ask_at = stage == 0 ? S - 1 : stage - 1;         // the stage that the step before has left
+    ask(ask_at);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    const uint8_t* src = ring + stage * K * kWarps * 32 * R;
+    const int h = at.h + sub;
+    uint64_t va[NS][H], vb[NS][H], ga[NS][H], gb[NS][H];
+    uint64_t sq = 0, sd = 0;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const bool on = h < at.h1 && has[s];
+#pragma unroll
+      for (int j = 0; j < H; ++j) va[s][j] = vb[s][j] = ga[s][j] = gb[s][j] = 0;
+      if (on) {
+        Run<T, P> lo, hi;
+        lo.read(src + (s * (K / NS)) * kWarps * 32 * R);
+        hi.read(src + (s * (K / NS) + 1) * kWarps * 32 * R);
+        take<T, P>(lo, hi, inter, va[s], vb[s]);
+        if (BWD) {
+          lo.read(src + (s * (K / NS) + 2) * kWarps * 32 * R);
+          hi.read(src + (s * (K / NS) + 3) * kWarps * 32 * R);
+          take<T, P>(lo, hi, inter, ga[s], gb[s]);
+          if (un[s].pair >= 0) {
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              const uint64_t u = fma2(gb[s][j], sn[s][j], mul2(ga[s][j], c[s][j]));
+              gb[s][j] = fma2(neg2(ga[s][j]), sn[s][j], mul2(gb[s][j], c[s][j]));
+              ga[s][j] = u;
+            }
+          }
+        }
+      }
+      if (norm) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          sq = fma2(va[s][j], va[s][j], sq);
+          sq = fma2(vb[s][j], vb[s][j], sq);
+          if (BWD) {
+            sd = fma2(mul2(ga[s][j], wa[s][j]), va[s][j], sd);
+            sd = fma2(mul2(gb[s][j], wb[s][j]), vb[s][j], sd);
+          }
+        }
+      }
+    }
+    float rn = 1.f, k = 0.f;
+    if (norm) {
+      const float2 q2 = untwo(sq), d2 = untwo(sd);
+      rn = rsqrtf(row_sum<L>(q2.x + q2.y) * inv_dim + p.eps);
+      if (BWD) k = row_sum<L>(d2.x + d2.y) * inv_dim * rn * rn * rn;
+    }
+    const uint64_t rn2 = two(rn, rn), k2 = two(-k, -k);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if (!(h < at.h1 && has[s])) continue;
+      uint64_t oa[H], ob[H];
 #pragma unroll
       for (int j = 0; j < H; ++j) {
-        c[s][j] = two(1.f, 1.f);
-        sn[s][j] = 0;
-        if (un[s].pair >= 0) {
-          const float2 u = cs[un[s].pair + (inter ? j : 2 * j)], v = cs[un[s].pair + (inter ? j + H : 2 * j + 1)];
-          c[s][j] = two(u.x, v.x);
-          sn[s][j] = two(u.y, v.y);
+        if (BWD && norm) {
+          da[s][j] = fma2(ga[s][j], mul2(va[s][j], rn2), da[s][j]);
+          db[s][j] = fma2(gb[s][j], mul2(vb[s][j], rn2), db[s][j]);
+          oa[j] = fma2(va[s][j], k2, mul2(mul2(ga[s][j], wa[s][j]), rn2));
+          ob[j] = fma2(vb[s][j], k2, mul2(mul2(gb[s][j], wb[s][j]), rn2));
+        } else if (BWD) {
+          oa[j] = ga[s][j];
+          ob[j] = gb[s][j];
+        } else {
+          oa[j] = norm ? mul2(mul2(va[s][j], rn2), wa[s][j]) : va[s][j];
+          ob[j] = norm ? mul2(mul2(vb[s][j], rn2), wb[s][j]) : vb[s][j];
         }
       }
-#pragma unroll 1
-    for (int hb = h0; hb < h1; hb += RPW * U) {
-      Run<T, P> xl[U][NS], xh[U][NS], gl[U][NS], gh[U][NS];
+      if (!BWD && un[s].pair >= 0) {
 #pragma unroll
-      for (int r = 0; r < U; ++r) {
-        const int h = hb + r * RPW + sub;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-          if (h < h1 && has[s]) {
-            xl[r][s].load(x + h * t.x_sh + un[s].lo);
-            xh[r][s].load(x + h * t.x_sh + un[s].hi);
-            if (BWD) {
-              gl[r][s].load(dy + h * t.dy_sh + un[s].lo);
-              gh[r][s].load(dy + h * t.dy_sh + un[s].hi);
-            }
-          }
+        for (int j = 0; j < H; ++j) {
+          const uint64_t u = fma2(neg2(ob[j]), sn[s][j], mul2(oa[j], c[s][j]));
+          ob[j] = fma2(oa[j], sn[s][j], mul2(ob[j], c[s][j]));
+          oa[j] = u;
+        }
       }
-#pragma unroll
-      for (int r = 0; r < U; ++r) {
-        const int h = hb + r * RPW + sub;
-        uint64_t va[NS][H], vb[NS][H], ga[NS][H], gb[NS][H];
-        uint64_t sq = 0, sd = 0;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          const bool on = h < h1 && has[s];
-#pragma unroll
-          for (int j = 0; j < H; ++j) va[s][j] = vb[s][j] = ga[s][j] = gb[s][j] = 0;
-          if (on) {
-            take<T, P>(xl[r][s], xh[r][s], inter, va[s], vb[s]);
-            if (BWD) {
-              take<T, P>(gl[r][s], gh[r][s], inter, ga[s], gb[s]);
-              if (un[s].pair >= 0) {
-#pragma unroll
-                for (int j = 0; j < H; ++j) {
-                  const uint64_t u = fma2(gb[s][j], sn[s][j], mul2(ga[s][j], c[s][j]));
-                  gb[s][j] = fma2(neg2(ga[s][j]), sn[s][j], mul2(gb[s][j], c[s][j]));
-                  ga[s][j] = u;
-                }
-              }
-            }
-          }
-          if (norm) {
-#pragma unroll
-            for (int j = 0; j < H; ++j) {
-              sq = fma2(va[s][j], va[s][j], sq);
-              sq = fma2(vb[s][j], vb[s][j], sq);
-              if (BWD) {
-                sd = fma2(mul2(ga[s][j], wa[s][j]), va[s][j], sd);
-                sd = fma2(mul2(gb[s][j], wb[s][j]), vb[s][j], sd);
-              }
-            }
-          }
-        }
-        float rn = 1.f, k = 0.f;
-        if (norm) {
-          const float2 q2 = untwo(sq), d2 = untwo(sd);
-          rn = rsqrtf(row_sum<L>(q2.x + q2.y) * inv_dim + p.eps);
-          if (BWD) k = row_sum<L>(d2.x + d2.y) * inv_dim * rn * rn * rn;
-        }
-        const uint64_t rn2 = two(rn, rn), k2 = two(-k, -k);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          if (!(h < h1 && has[s])) continue;
-          uint64_t oa[H], ob[H];
-#pragma unroll
-          for (int j = 0; j < H; ++j) {
-            if (BWD && norm) {
-              da[s][j] = fma2(ga[s][j], mul2(va[s][j], rn2), da[s][j]);
-              db[s][j] = fma2(gb[s][j], mul2(vb[s][j], rn2), db[s][j]);
-              oa[j] = fma2(va[s][j], k2, mul2(mul2(ga[s][j], wa[s][j]), rn2));
-              ob[j] = fma2(vb[s][j], k2, mul2(mul2(gb[s][j], wb[s][j]), rn2));
-            } else if (BWD) {
-              oa[j] = ga[s][j];
-              ob[j] = gb[s][j];
-            } else {
-              oa[j] = norm ? mul2(mul2(va[s][j], rn2), wa[s][j]) : va[s][j];
-              ob[j] = norm ? mul2(mul2(vb[s][j], rn2), wb[s][j]) : vb[s][j];
-            }
-          }
-          if (!BWD && un[s].pair >= 0) {
-#pragma unroll
-            for (int j = 0; j < H; ++j) {
-              const uint64_t u = fma2(neg2(ob[j]), sn[s][j], mul2(oa[j], c[s][j]));
-              ob[j] = fma2(oa[j], sn[s][j], mul2(ob[j], c[s][j]));
-              oa[j] = u;
-            }
-          }
-          if (stored) {
-            Run<T, P> lo, hi;
-            give<T, P>(oa, ob, inter, lo, hi);
-            lo.store(y + h * y_sh + un[s].lo);
-            hi.store(y + h * y_sh + un[s].hi);
-          }
-        }
+      if (stored) {
+        Run<T, P> lo, hi;
+        give<T, P>(oa, ob, inter, lo, hi);
+        lo.store(y + h * y_sh + un[s].lo);
+        hi.store(y + h * y_sh + un[s].hi);
       }
     }
+    if (++stage == S) stage = 0;
+    have = at.next(RPW, fresh);
   }
 
   if (BWD && t.dweight != nullptr) {
     // the CTA's sum of each column, rows in a fixed order
-    float* part = reinterpret_cast<float*>(steps);             // [kWarps][dim], over the turns
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float* part = reinterpret_cast<float*>(smem);              // [kWarps][dim], over the ring
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -612,6 +691,10 @@ static Shape shape_of(const SfaRotaryParams& p, bool bwd) {
 
 // Items of up to 32 warp steps share one token's cosines; fewer when there would
 // be too few items to fill the SMs (a decode step), down to one step each.
+// The CTAs are shared out by work, an item's cosines counted as four steps: by heads alone, the few CTAs of
+// a lone kv head ran 100 us behind the others.  Two CTAs per SM where each warp has few items (5003 tokens of
+// 10 + 2 heads: 40 us, against 47 with eight), up to eight where that leaves it four (559 against 646 us
+// for 32768 tokens), so that the SMs finish together.
 static Grid make_grid(const SfaRotaryParams& p, const Shape& s) {
   Grid g{};
   const int sms = device_sm_count(), rpw = s.p ? 32 / s.lanes : 1;
@@ -619,13 +702,21 @@ static Grid make_grid(const SfaRotaryParams& p, const Shape& s) {
   int64_t heads = 0;
   for (int i = 0; i < p.num_tensors; ++i) heads += p.t[i].heads;
   const int64_t steps = std::max<int64_t>(1, tokens * ((heads + rpw - 1) / rpw));
-  const int per = (int)std::min<int64_t>(32, std::max<int64_t>(1, steps / ((int64_t)sms * 32)));
-  const int most = sms * 8;
+  const int per = (int)std::min<int64_t>(32, std::max<int64_t>(1, steps / ((int64_t)sms * 8)));
+  int64_t cost[3], total = 0;
   for (int i = 0; i < p.num_tensors; ++i) {
     g.heads_per[i] = s.p ? std::min(p.t[i].heads, per * rpw) : 1;
     g.chunks[i] = (p.t[i].heads + g.heads_per[i] - 1) / g.heads_per[i];
+    cost[i] = (p.t[i].heads + rpw - 1) / rpw + 4 * g.chunks[i];
+    total += cost[i];
+  }
+  int64_t items = 0;
+  for (int i = 0; i < p.num_tensors; ++i) items += tokens * g.chunks[i];
+  const int64_t most =
+      sms * std::min<int64_t>(8, std::max<int64_t>(2, items / ((int64_t)sms * kWarps * 4)));
+  for (int i = 0; i < p.num_tensors; ++i) {
     const int64_t ctas = (tokens * g.chunks[i] + kWarps - 1) / kWarps;
-    const int64_t share = std::max<int64_t>(1, most * (int64_t)p.t[i].heads / heads);
+    const int64_t share = std::max<int64_t>(1, most * cost[i] / total);
     g.ctas[i] = (int)std::min(ctas, share);
   }
   return g;
@@ -637,19 +728,22 @@ static int total_ctas(const SfaRotaryParams& p, const Grid& g) {
   return n;
 }
 
+template <typename T, int P, int L, int NS, bool BWD>
+static void launch_shape(const SfaRotaryParams& p, const Grid& g, cudaStream_t st) {
+  const size_t turns = (size_t)(p.rot / 2) * (sizeof(uint64_t) + kWarps * sizeof(float2));   // at most 36 KB
+  const size_t smem = std::max(ring_bytes<T, P, NS, BWD>() + turns, BWD ? kWarps * sizeof(float) * p.dim : (size_t)0);
+  if (smem > 48 * 1024)
+    cudaFuncSetAttribute(rotary_kernel<T, P, L, NS, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  rotary_kernel<T, P, L, NS, BWD><<<total_ctas(p, g), kWarps * 32, smem, st>>>(p, g);
+}
+
 template <typename T, int P, bool BWD>
 static void launch_runs(const SfaRotaryParams& p, const Grid& g, const Shape& s, cudaStream_t st) {
-  const int n = total_ctas(p, g), threads = kWarps * 32;
-  const size_t smem = std::max((size_t)(p.rot / 2) * (sizeof(uint64_t) + kWarps * sizeof(float2)),   // at most 36 KB
-                               BWD ? kWarps * sizeof(float) * p.dim : (size_t)0);
-  if (s.units == 1) {
-    if (s.lanes == 4) rotary_kernel<T, P, 4, 1, BWD><<<n, threads, smem, st>>>(p, g);
-    else if (s.lanes == 8) rotary_kernel<T, P, 8, 1, BWD><<<n, threads, smem, st>>>(p, g);
-    else if (s.lanes == 16) rotary_kernel<T, P, 16, 1, BWD><<<n, threads, smem, st>>>(p, g);
-    else rotary_kernel<T, P, 32, 1, BWD><<<n, threads, smem, st>>>(p, g);
-  } else {
-    rotary_kernel<T, P, 32, P == 8 ? 2 : 4, BWD><<<n, threads, smem, st>>>(p, g);   // above 512 (256) dims
-  }
+  if (s.units > 1) return launch_shape<T, P, 32, P == 8 ? 2 : 4, BWD>(p, g, st);   // above 512 (256) dims
+  if (s.lanes == 4) return launch_shape<T, P, 4, 1, BWD>(p, g, st);
+  if (s.lanes == 8) return launch_shape<T, P, 8, 1, BWD>(p, g, st);
+  if (s.lanes == 16) return launch_shape<T, P, 16, 1, BWD>(p, g, st);
+  launch_shape<T, P, 32, 1, BWD>(p, g, st);
 }
 
 template <typename T, bool BWD>
