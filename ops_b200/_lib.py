@@ -185,8 +185,9 @@ def packer(cls):
 
 
 def stream_of(device: torch.device) -> int:
-    """Handle of the device's current stream."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the device's current stream, without the stream object that
+    ``torch.cuda.current_stream`` makes (2.3 us a call, against 0.1)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class on:

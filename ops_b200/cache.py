@@ -15,7 +15,6 @@ page_size, ...]`` with contiguous pages: K and V of every layer, any type.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 from typing import Optional, Sequence
 
@@ -38,27 +37,27 @@ def _ints(name: str, t: torch.Tensor, dim: int, like: torch.Tensor, size: Option
 def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Optional[int]):
     if len(pools) == 0:
         raise ValueError("pools must hold at least one tensor")
-    first = pools[0]
+    lead, device = pools[0].shape[:2], like.device
+    bad = len(lead) < 2 or lead[1] < 1 or num_pages not in (None, lead[0])
     values = []
     for t in pools:
-        if t.dim() < 2 or t.device != like.device or t.shape[1] < 1 or t.shape[:2] != first.shape[:2] or (
-                num_pages is not None and t.shape[0] != num_pages):
+        if bad or t.shape[:2] != lead or t.device != device:
             raise ValueError("every pool must be [num_pages, page_size, ...] with the same pages, on the device of the table")
+        size = t.element_size()
         if t.is_contiguous():
-            inner = expect = math.prod(t.shape[1:])
+            inner = expect = t.numel() // max(lead[0], 1)
         else:
             inner = t.stride(0) if t.shape[0] > 1 else 0
             expect = 1
-            for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-                if size > 1 and stride != expect:
+            for extent, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+                if extent > 1 and stride != expect:
                     raise ValueError("a pool's pages must be contiguous")
-                expect *= size
+                expect *= extent
             if t.shape[0] > 1 and inner < expect:
                 raise ValueError("a pool's pages must not overlap")
-        size = t.element_size()
         values += (t.data_ptr(), (inner or expect) * size, expect * size)
     arr = (SfaCachePool * len(pools)).from_buffer_copy(struct.pack("@" + "Pqq" * len(pools), *values))
-    return arr, first.shape[0], first.shape[1]
+    return arr, lead[0], lead[1]
 
 
 _pack = _lib.packer(SfaCacheParams)
@@ -83,7 +82,7 @@ def _call(name: str, P: SfaCacheParams, like: torch.Tensor, workspace: bool = Tr
     with _lib.on(like.device):
         if workspace:
             nbytes = lib.sfa_cache_workspace_bytes(ctypes.byref(P))
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=like.device)
+            ws = like.new_empty(max(nbytes, 1), dtype=torch.uint8)
             rc = getattr(lib, name)(ctypes.byref(P), ws.data_ptr(), nbytes, _lib.stream_of(like.device))
         else:
             rc = getattr(lib, name)(ctypes.byref(P), _lib.stream_of(like.device))

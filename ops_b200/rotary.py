@@ -110,10 +110,12 @@ def _check_turn(x: torch.Tensor, positions, frequencies, interleaved, start, eps
             raise ValueError("positions must be int32 or int64 on the inputs' device")
         rot = 2 * frequencies.numel()
         frequencies = frequencies.contiguous()
-        try:
-            positions = positions.expand(x.shape[:-2])
-        except RuntimeError:
-            raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to tokens {tuple(x.shape[:-2])}")
+        tokens = x.shape[:-2]
+        if positions.shape != tokens:
+            try:
+                positions = positions.expand(tokens)
+            except RuntimeError:
+                raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to tokens {tuple(tokens)}")
     if start < 0 or start + rot > x.shape[-1]:
         raise ValueError("the rotated dims [start, start + rotary_dim) must lie within the head")
     if not eps >= 0:
@@ -165,10 +167,10 @@ def _params(x: torch.Tensor, tensors, cfg: _Cfg, positions, frequencies, cache=_
 class _NormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, frequencies, cfg: _Cfg):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        oq = torch.empty_like(q, memory_format=torch.contiguous_format)
         tensors = [_tensor(q, wq, oq)]
         if k is not None:
-            ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            ok = torch.empty_like(k, memory_format=torch.contiguous_format)
             tensors.append(_tensor(k, wk, ok))
         P = _params(q, tensors, cfg, positions, frequencies)
         with _lib.on(q.device):
@@ -189,7 +191,7 @@ class _NormRotary(torch.autograd.Function):
             if x is None or not (need[i] or need[2 + i]):
                 continue
             dy = _rows(grads[i])
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dx = torch.empty_like(x, memory_format=torch.contiguous_format)
             dw = torch.empty_like(w) if w is not None and need[2 + i] else None
             tensors.append(_tensor(x, w, None, dy, dx, dw))
             out[i], out[2 + i] = dx, dw
@@ -301,7 +303,7 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
     lens = cache_seqlens.contiguous()
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     cache = (table.data_ptr(), lens.data_ptr(), 0 if cu is None else cu.data_ptr(), table.stride(0))
     sizes = (n, k_cache.shape[0], k_cache.shape[1], table.shape[1])
     tensors = [_tensor(q, wq, out), _paged(k, wk, k_cache, _TURN), _paged(v, None, v_cache, 0)]

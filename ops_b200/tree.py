@@ -93,8 +93,8 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     par = None if parents is None else parents.contiguous()
     sink = None if attn_sink is None else attn_sink.detach().float().contiguous()
     hq, dv = q.shape[1], v_cache.shape[3]
-    o = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
-    lse = torch.empty(total, hq, dtype=torch.float32, device=device)
+    o = q.new_empty((total, hq, dv))
+    lse = q.new_empty((total, hq), dtype=torch.float32)
     pages, page, hk = k_cache.shape[:3]
     ks, vs = k_cache.stride(), v_cache.stride()
     width = table.shape[1]
@@ -108,6 +108,6 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     lib, at = _lib.load(), ctypes.byref(P)
     with _lib.on(device):
         nbytes = lib.sfa_tree_workspace_bytes(at)                       # 0 also when the call is refused
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        ws = q.new_empty(max(nbytes, 1), dtype=torch.uint8)
         _lib.check(lib.sfa_tree_attention(at, ws.data_ptr(), nbytes, _lib.stream_of(device)), "sfa_tree_attention")
     return o, lse
