@@ -56,6 +56,9 @@ def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Op
             if t.shape[0] > 1 and inner < expect:
                 raise ValueError("a pool's pages must not overlap")
         values += (t.data_ptr(), (inner or expect) * size, expect * size)
+    held = [ptr for ptr in values[::3] if ptr]
+    if len(set(held)) < len(held):
+        raise ValueError("a pool is named twice")
     arr = (SfaCachePool * len(pools)).from_buffer_copy(struct.pack("@" + "Pqq" * len(pools), *values))
     return arr, lead[0], lead[1]
 
@@ -92,6 +95,8 @@ def _call(name: str, P: SfaCacheParams, like: torch.Tensor, workspace: bool = Tr
 def _state(refcounts, block_table, cache_seqlens, page_size=None) -> None:
     _ints("refcounts", refcounts, 1, refcounts)
     _ints("block_table", block_table, 2, refcounts)
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table's rows must not overlap")
     if cache_seqlens is not None:
         _ints("cache_seqlens", cache_seqlens, 1, refcounts, block_table.shape[0])
     if page_size is not None and int(page_size) < 1:

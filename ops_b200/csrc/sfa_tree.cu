@@ -539,36 +539,48 @@ __device__ __forceinline__ void store4(T* at, float4 v) {
   *reinterpret_cast<uint2*>(at) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
 }
 
+template <typename T>
+__device__ __forceinline__ void empty_row(const SfaTreeParams& p, int64_t row, int head, int grp) {
+  store4<T>(static_cast<T*>(p.o) + row * p.o_st + (int64_t)head * p.o_sh + grp * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+  if (grp == 0) p.lse[row * p.l_st + (int64_t)head * p.l_sh] = p.attn_sink ? __ldg(p.attn_sink + head) : -INFINITY;
+}
+
+// Rows before the first and behind the last sequence, then of each sequence past the tiles (max_q was too small).
+template <typename T>
+static __device__ __noinline__ void rows_of_no_tile(const Args& a, int first, int step) {
+  const SfaTreeParams& p = a.p;
+  const int n = p.num_seqs, groups = p.d_v / 4;
+  const int begin = n > 0 && p.cu_seqlens ? min(p.total_q, max(0, __ldg(p.cu_seqlens))) : 0;
+  const int end = n == 0 ? 0 : p.cu_seqlens ? max(begin, __ldg(p.cu_seqlens + n)) : n;
+  const int64_t todo = (int64_t)(begin + max(0, p.total_q - end)) * p.h_q * groups;
+#pragma unroll 1
+  for (int64_t i = first; i < todo; i += step) {
+    const int64_t row = i / (groups * p.h_q);
+    empty_row<T>(p, row < begin ? row : end + (row - begin), (int)(i / groups % p.h_q), (int)(i % groups));
+  }
+  if (!p.cu_seqlens) return;
+  const int covered = a.ntiles / a.n_hg * a.NT;
+#pragma unroll 1
+  for (int s = first; s < n; s += step) {
+    const int q0 = __ldg(p.cu_seqlens + s), q1 = min(p.total_q, __ldg(p.cu_seqlens + s + 1));
+#pragma unroll 1
+    for (int row = q0 < 0 ? q1 : q0 + covered; row < q1; ++row)
+#pragma unroll 1
+      for (int i = 0; i < p.h_q * groups; ++i) empty_row<T>(p, row, i / groups, i % groups);
+  }
+}
+
 // Joins the pieces of units that several ranges share, in range order; also
-// writes the rows nothing else does: of sequences without keys, behind the last
-// sequence, and past max_q.  Item = (row of a tile, four dims).
+// writes the rows nothing else does: of sequences without keys, outside all
+// sequences, and past max_q.  Item = (row of a tile, four dims).
 template <typename T>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Args a, int tile_rows) {
   const SfaTreeParams& p = a.p;
   const int n = p.num_seqs, units = n * p.h_kv * a.ntiles;
   const int groups = p.d_v / 4;
   T* out = static_cast<T*>(p.o);
-  auto empty_row = [&](int64_t row, int head, int grp) {
-    store4<T>(out + row * p.o_st + (int64_t)head * p.o_sh + grp * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (grp == 0) p.lse[row * p.l_st + (int64_t)head * p.l_sh] = p.attn_sink ? __ldg(p.attn_sink + head) : -INFINITY;
-  };
   const int first = blockIdx.y * blockDim.x + threadIdx.x, step = gridDim.y * blockDim.x;
-  if ((int)blockIdx.x >= units) {
-    // rows behind the last sequence, then of each sequence past the tiles (max_q was too small)
-    const int end = n == 0 ? 0 : p.cu_seqlens ? max(0, __ldg(p.cu_seqlens + n)) : n;
-    const int64_t todo = (int64_t)max(0, p.total_q - end) * p.h_q * groups;
-    for (int64_t i = first; i < todo; i += step)
-      empty_row(end + i / (groups * p.h_q), (int)(i / groups % p.h_q), (int)(i % groups));
-    if (p.cu_seqlens) {
-      const int covered = a.ntiles / a.n_hg * a.NT;
-      for (int s = first; s < n; s += step) {
-        const int q0 = __ldg(p.cu_seqlens + s), q1 = min(p.total_q, __ldg(p.cu_seqlens + s + 1));
-        for (int row = q0 + covered; row < q1; ++row)
-          for (int i = 0; i < p.h_q * groups; ++i) empty_row(row, i / groups, i % groups);
-      }
-    }
-    return;
-  }
+  if ((int)blockIdx.x >= units) return rows_of_no_tile<T>(a, first, step);
   const int tile = blockIdx.x % a.ntiles, h = blockIdx.x / a.ntiles % p.h_kv, s = blockIdx.x / a.ntiles / p.h_kv;
   const int c0 = a.cum[s], nch = a.cum[s + 1] - c0;
   const int line = a.cum[n] * p.h_kv, len = max(a.min_chunks, (line + a.ranges - 1) / a.ranges);
@@ -577,6 +589,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   if (nch > 0 && r0 == r1) return;
   const Seq q = load_seq(a, s);
   const int node0 = tile / a.n_hg * a.NT;
+#pragma unroll 1
   for (int i = first; i < tile_rows * groups; i += step) {
     const int m = i % tile_rows, grp = i / tile_rows;
     const int node = node0 + (a.n_hg > 1 ? 0 : m / a.GB);
@@ -585,7 +598,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
     const int head = h * a.G + hh;
     const int64_t row = q.q0 + node;
     if (nch == 0) {
-      empty_row(row, head, grp);
+      empty_row<T>(p, row, head, grp);
       continue;
     }
     auto slot = [&](int r) { return part_slot(a, r, tile, r == r0); };
@@ -641,6 +654,10 @@ static int check(const SfaTreeParams* p) {
   const int64_t chunks = ((int64_t)p->table_width * p->page_size + kKeys - 1) / kKeys;
   if (chunks * p->num_seqs * p->h_kv >= INT32_MAX || (int64_t)p->table_width * p->page_size >= INT32_MAX)
     return report_error(SFA_ERR_UNSUPPORTED, "tree attention: table too large");
+  const int g = p->h_q / p->h_kv, per_tile = g > 128 ? 1 : 128 / g;         // rows and head tiles of a tile
+  const int64_t tiles = ((int64_t)std::max(1, p->cu_seqlens ? p->max_q : 1) + per_tile - 1) / per_tile * ((g + 127) / 128);
+  if (tiles > 65535 || tiles * p->num_seqs * p->h_kv >= INT32_MAX)
+    return report_error(SFA_ERR_UNSUPPORTED, "tree attention: too many drafted rows a sequence for one call");
   if (p->total_q == 0) return SFA_OK;
   if (!p->q || !p->o || !p->lse) return bad("q, o and lse must be non-NULL");
   if (p->num_seqs > 0 && ((p->table_width > 0 && !p->block_table) || !p->cache_seqlens))

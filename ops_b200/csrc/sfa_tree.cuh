@@ -56,7 +56,7 @@ static __device__ __noinline__ Seq load_seq(const Args& a, int s) {
   const int len = __ldg(p.cache_seqlens + s);
   if (p.cu_seqlens) {
     r.q0 = __ldg(p.cu_seqlens + s);
-    r.rows = max(0, __ldg(p.cu_seqlens + s + 1) - r.q0);
+    r.rows = r.q0 < 0 ? 0 : max(0, __ldg(p.cu_seqlens + s + 1) - r.q0);
   } else {
     r.q0 = s;
     r.rows = 1;

@@ -108,6 +108,8 @@ def _check_turn(x: torch.Tensor, positions, frequencies, interleaved, start, eps
             raise ValueError("frequencies must be a 1-D float64 tensor on the inputs' device")
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != x.device:
             raise ValueError("positions must be int32 or int64 on the inputs' device")
+        if frequencies.requires_grad:
+            raise ValueError("frequencies have no gradient: detach them")
         rot = 2 * frequencies.numel()
         frequencies = frequencies.contiguous()
         tokens = x.shape[:-2]
@@ -289,6 +291,8 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
             raise ValueError(f"{name} must have the type, heads and head size of the rows stored into it")
     if v_cache.shape[:2] != k_cache.shape[:2]:
         raise ValueError("k_cache and v_cache must have the same pages")
+    if k_cache.data_ptr() == v_cache.data_ptr() != 0:
+        raise ValueError("k_cache and v_cache must not be the same memory")
     _check_table(block_table, cache_seqlens, q)
     n = block_table.shape[0]
     if cu_seqlens is None:

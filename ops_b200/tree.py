@@ -50,7 +50,7 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     where a drafted row's ancestors are token indices).  A table entry outside
     the pool holds no keys.  Cache rows that a row does not see have no effect
     on it, whatever they hold.  A row that sees nothing gives ``o = 0`` and
-    ``lse = -inf`` (or its sink); so do rows behind ``cu_seqlens[n]``.
+    ``lse = -inf`` (or its sink); so do rows outside all sequences.
 
     ``max_seqlen_q`` must cover the longest sequence of drafted rows; left unset
     with ``cu_seqlens`` it is read back with a host sync.  ``max_seqlen_k`` is an
@@ -85,6 +85,7 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError("the inputs must be CUDA tensors (tree attention has no CPU implementation)")
     if max_seqlen_q is None:
         max_seqlen_q = int((cu_seqlens[1:] - cu_seqlens[:-1]).max().item()) if n else 0
+    max_seqlen_q = min(int(max_seqlen_q), max(1, total))            # no sequence has more rows
     device = q.device
     q = q if _tma_ready(q) else q.detach().clone(memory_format=torch.contiguous_format)
     table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
@@ -98,12 +99,11 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     pages, page, hk = k_cache.shape[:3]
     ks, vs = k_cache.stride(), v_cache.stride()
     width = table.shape[1]
-    if max_seqlen_k is None:
-        max_seqlen_k = min(2**31 - 1, width * page)
+    max_seqlen_k = min(2**31 - 1, width * page if max_seqlen_k is None else int(max_seqlen_k))
     P = _pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),
               0 if cu is None else cu.data_ptr(), 0 if par is None else par.data_ptr(),
               0 if sink is None else sink.data_ptr(), o.data_ptr(), lse.data_ptr(), q.stride(0), q.stride(1), ks[1], ks[2],
-              vs[1], vs[2], hq * dv, dv, hq, 1, table.stride(0), n, total, int(max_seqlen_q), int(max_seqlen_k), hq, hk,
+              vs[1], vs[2], hq * dv, dv, hq, 1, table.stride(0), n, total, max_seqlen_q, max_seqlen_k, hq, hk,
               q.shape[2], dv, pages, page, width, _DTYPE[q.dtype], float(scale), 0)
     lib, at = _lib.load(), ctypes.byref(P)
     with _lib.on(device):

@@ -72,6 +72,18 @@ def test_refusals(op, bad, msg, ops):
         CALLS[op]({**GOOD, **bad})
 
 
+def test_what_would_be_moved_twice_is_refused():
+    one = pool(6, 8, 2)
+    for op in ("fork", "accept", "compact", "copy"):
+        with pytest.raises(ValueError, match="twice"):
+            CALLS[op]({**GOOD, "pools": [one, pool(6, 8, 5), one]})
+        with pytest.raises(ValueError, match="CUDA"):                      # nothing in them: nothing moves
+            CALLS[op]({**GOOD, "pools": [pool(6, 8, 0), pool(6, 8, 0)]})
+    for op in ("reserve", "trim", "fork", "compact"):
+        with pytest.raises(ValueError, match="overlap"):
+            CALLS[op]({**GOOD, "table": ints(1, 4).expand(3, 4)})
+
+
 def test_page_size_is_checked():
     for f in (ops_b200.paged_cache_reserve, ops_b200.paged_cache_trim):
         with pytest.raises(ValueError, match="page_size"):

@@ -178,6 +178,21 @@ def test_missing_pages_short_caches_and_rows_behind():
     assert empty[0].shape == (0, 8, 64)
 
 
+def test_rows_before_the_first_sequence_and_bad_offsets():
+    q, kc, vc, table, lens, par, cu = problem([3, 70, 2], [90, 130, 40], 8, 2, 64, 64, 16, torch.bfloat16, 21, behind=4)
+    want = run(q, kc, vc, table, lens, par, cu)
+    front = 3
+    q2, par2 = torch.cat([q[:front], q]), torch.cat([par[:front], par])
+    got = run(q2, kc, vc, table, lens, par2, cu + front, max_seqlen_q=70, max_seqlen_k=2 ** 40)
+    assert not got[0][:front].any() and torch.isinf(got[1][:front]).all()
+    assert torch.equal(got[0][front:], want[0]) and torch.equal(got[1][front:], want[1])
+    # offsets in front of the tensor name no rows; the other sequences are untouched by them
+    odd = cu.clone()
+    odd[0] = -5
+    got = run(q, kc, vc, table, lens, par, odd, max_seqlen_q=70)
+    assert torch.equal(got[0][3:], want[0][3:]) and torch.equal(got[1][3:], want[1][3:])
+
+
 def test_extreme_scores():
     # scores that rise by far more than a rescale allows from chunk to chunk, and fall; one key that takes all
     q, kc, vc, table, lens, par, cu = problem([4, 1], [700, 300], 8, 2, 64, 64, 64, torch.bfloat16, 4, fill=0.0)

@@ -76,10 +76,14 @@ def good():
     (dict(frequencies=torch.zeros(16)), "float64"), (dict(start=33), "within the head"), (dict(start=-1), "within the head"),
     (dict(q_weight=torch.ones(32)), "q_weight"), (dict(k_weight=torch.ones(64, dtype=torch.int64)), "k_weight"),
     (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(frequencies=torch.zeros(16, dtype=torch.float64, requires_grad=True)), "no gradient"),
 ])
 def test_refusals(bad, msg):
     with pytest.raises(ValueError, match=msg):
         ops_b200.qk_norm_rotary(**{**good(), **bad})
+
+
+ONE_POOL = torch.zeros(5, 8, 2, 64)
 
 
 def append_args():
@@ -93,7 +97,7 @@ def append_args():
 @pytest.mark.parametrize("bad,msg", [
     (dict(), "CUDA"), (dict(v=torch.zeros(2, 2, 64)), "v must be"), (dict(v=torch.zeros(3, 1, 64)), "k's heads"),
     (dict(k_cache=torch.zeros(5, 8, 2, 64).half()), "k_cache"), (dict(v_cache=torch.zeros(5, 8, 2, 32)), "v_cache"),
-    (dict(v_cache=torch.zeros(4, 8, 2, 64)), "same pages"),
+    (dict(v_cache=torch.zeros(4, 8, 2, 64)), "same pages"), (dict(k_cache=ONE_POOL, v_cache=ONE_POOL), "same memory"),
     (dict(k_cache=torch.zeros(5, 2, 8, 64).transpose(1, 2)), "row ranges"),
     (dict(block_table=torch.zeros(3, 2)), "int32"), (dict(cache_seqlens=torch.ones(2, dtype=torch.int32)), "same number"),
     (dict(block_table=torch.zeros(2, 2, dtype=torch.int32), cache_seqlens=torch.ones(2, dtype=torch.int32)), "one row"),

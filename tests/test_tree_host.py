@@ -70,6 +70,8 @@ def params(**kw):
     (dict(block_table=None), "INVALID_ARGUMENT", "block_table"), (dict(k_st=124), "INVALID_ARGUMENT", "strides"),
     (dict(q_sh=0), "INVALID_ARGUMENT", "strides"), (dict(v=0x10008), "INVALID_ARGUMENT", "aligned"),
     (dict(num_pages=2 ** 30, page_size=2), "UNSUPPORTED", "rows"), (dict(table_width=2 ** 30, page_size=64), "UNSUPPORTED", "table"),
+    (dict(max_q=32 * 65535 + 1), "UNSUPPORTED", "too many drafted rows"),
+    (dict(num_seqs=2 ** 15, max_q=32 * 40000, table_width=1), "UNSUPPORTED", "too many drafted rows"),
     (dict(num_seqs=-1), "INVALID_ARGUMENT", "sizes"), (dict(cu_seqlens=None, total_q=1), "INVALID_ARGUMENT", "one row"),
 ])
 def test_c_abi_refusals(bad, code, msg):
