@@ -1,4 +1,4 @@
-// sfa_tree.cuh — what the two kernels of sfa_tree.cu and sfa_tree_pair.cu share:
+// sfa_tree.cuh — what the kernels of sfa_tree.cu, sfa_tree_pair.cu and sfa_tree_wide.cu share:
 // the arguments, how the chunk line of all sequences is cut into ranges, and the
 // walk of a CTA over the units its range touches.
 #pragma once
@@ -20,7 +20,6 @@ using namespace tok;
 constexpr int kQSlab = 128 * 128;               // bytes of a 128-row x 64-dim Q slab
 constexpr int kMaxNodes = SFA_TREE_MAX_NODES;
 constexpr int kAncWords = kMaxNodes / 32 + 3;   // + 2 zero words behind, odd row stride
-constexpr float kRescaleLog2 = 8.f;
 
 struct Args {
   SfaTreeParams p;
@@ -36,7 +35,7 @@ struct Args {
   int dvp;           // d_v rounded up to 16
   int box, box_log;  // rows of a K / V box, a power of two
   int kst, vst;      // ring stages
-  uint32_t col_s, tmem_cols;
+  uint32_t tmem_cols;
   uint32_t off_k, off_v, off_sh;
   float* part_o;     // [range][tile][2][dvp / 4][128][4]
   float2* part_ml;   // [range][tile][2][128]  (m, l)
@@ -244,8 +243,11 @@ __device__ __forceinline__ int64_t part_slot(const Args& a, int range, int tile,
   return ((int64_t)range * a.ntiles + tile) * 2 + (begins ? 1 : 0);
 }
 
-// sfa_tree_pair.cu
+// sfa_tree_pair.cu and sfa_tree_wide.cu
 size_t pair_shared_bytes();
+size_t wide_shared_bytes();
+cudaError_t launch_wide(const Args& a, size_t smem, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        cudaStream_t st);
 cudaError_t launch_pair(const Args& a, size_t smem, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                         cudaStream_t st);
 
