@@ -72,17 +72,59 @@ static __device__ __noinline__ void rows_of_no_tile(const Args& a, int first, in
   }
 }
 
-// Joins the pieces of units that several ranges share, in range order; also
+// A row's pieces r0, r0 + step .. r1 of one tile, four dims: their maximum M (with the one given), sum and O.
+__device__ __forceinline__ void join_pieces(const Args& a, int tile, int m, int grp, int first_piece, int r0, int r1, int step,
+                                            float& M, float& lt, float4& o) {
+  auto slot = [&](int r) { return part_slot(a, r, tile, r == first_piece); };
+#pragma unroll 1
+  for (int r = r0; r <= r1; r += 4 * step) {                  // four loads under way
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = r + k * step <= r1 ? a.part_ml[slot(r + k * step) * 128 + m].x : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, v[k]);
+  }
+#pragma unroll 1
+  for (int r = r0; r <= r1; r += 4 * step) {
+    float2 ml[4];
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = slot(r + k * step <= r1 ? r + k * step : r);
+      ml[k] = a.part_ml[at * 128 + m];
+      v[k] = reinterpret_cast<const float4*>(a.part_o)[(at * (a.dvp / 4) + grp) * 128 + m];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // past the last piece, or a piece that holds no key of this row
+      if (r + k * step > r1 || (ml[k].x == -INFINITY && ml[k].y == 0.f)) continue;
+      const float w = ex2(ml[k].x - M);
+      lt = fmaf(ml[k].y, w, lt);
+      o.x = fmaf(v[k].x, w, o.x);
+      o.y = fmaf(v[k].y, w, o.y);
+      o.z = fmaf(v[k].z, w, o.z);
+      o.w = fmaf(v[k].w, w, o.w);
+    }
+  }
+}
+
+// Joins the pieces of units that several ranges share, in a fixed order; also
 // writes the rows nothing else does: of sequences without keys, outside all
-// sequences, and past max_q.  Item = (row of a tile, four dims).
+// sequences, and past max_q.  Item = (row of a tile, four dims), a thread's work
+// while a unit has few pieces.  From 32 on (a long cache with few kv heads) the eight
+// warps of a CTA share the pieces of an item: with 74 pieces (256 dims, 131072 keys, two
+// kv heads) a call takes 77 us instead of 87; with 19 (128 dims, eight heads) it would
+// take 120 instead of 116.
+constexpr int kJoinWarps = 8, kManyPieces = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Args a, int tile_rows) {
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_combine_kernel(const __grid_constant__ Args a, int tile_rows) {
+  __shared__ float4 part_o[kJoinWarps][32];
+  __shared__ float2 part_ml[kJoinWarps][32];
   const SfaTreeParams& p = a.p;
   const int n = p.num_seqs, units = n * p.h_kv * a.ntiles;
   const int groups = p.d_v / 4;
-  T* out = static_cast<T*>(p.o);
-  const int first = blockIdx.y * blockDim.x + threadIdx.x, step = gridDim.y * blockDim.x;
-  if ((int)blockIdx.x >= units) return rows_of_no_tile<T>(a, first, step);
+  if ((int)blockIdx.x >= units)
+    return rows_of_no_tile<T>(a, blockIdx.y * blockDim.x + threadIdx.x, gridDim.y * blockDim.x);
   const int tile = blockIdx.x % a.ntiles, h = blockIdx.x / a.ntiles % p.h_kv, s = blockIdx.x / a.ntiles / p.h_kv;
   const int c0 = a.cum[s], nch = a.cum[s + 1] - c0;
   const int line = a.cum[n] * p.h_kv, len = max(a.min_chunks, (line + a.ranges - 1) / a.ranges);
@@ -91,39 +133,57 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   if (nch > 0 && r0 == r1) return;
   const Seq q = load_seq(a, s);
   const int node0 = tile / a.n_hg * a.NT;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool many = nch > 0 && r1 - r0 + 1 >= kManyPieces;
+  const int blocks = (tile_rows + 31) / 32;                   // of 32 rows
+  // many: a CTA an item of 32 rows and a group; else a warp
+  const int step = many ? gridDim.y : gridDim.y * kJoinWarps;
 #pragma unroll 1
-  for (int i = first; i < tile_rows * groups; i += step) {
-    const int m = i % tile_rows, grp = i / tile_rows;
+  for (int i = many ? blockIdx.y : blockIdx.y * kJoinWarps + warp; i < blocks * groups; i += step) {
+    const int m = i % blocks * 32 + lane, grp = i / blocks;
     const int node = node0 + (a.n_hg > 1 ? 0 : m / a.GB);
     const int hh = a.n_hg > 1 ? (tile % a.n_hg) * 128 + m : m % a.GB;
-    if (hh >= a.G || node >= q.rows || node - node0 >= a.NT || q.q0 + node >= p.total_q) continue;
+    const bool live = m < tile_rows && hh < a.G && node < q.rows && node - node0 < a.NT && q.q0 + node < p.total_q;
     const int head = h * a.G + hh;
     const int64_t row = q.q0 + node;
     if (nch == 0) {
-      empty_row<T>(p, row, head, grp);
+      if (live) empty_row<T>(p, row, head, grp);
       continue;
     }
-    auto slot = [&](int r) { return part_slot(a, r, tile, r == r0); };
-    const float s2 = p.attn_sink ? __ldg(p.attn_sink + head) * kLog2e : -INFINITY;
-    float M = s2;
-    for (int r = r0; r <= r1; ++r) M = fmaxf(M, a.part_ml[slot(r) * 128 + m].x);
-    float lt = s2 == -INFINITY ? 0.f : ex2(s2 - M);
+    const float s2 = p.attn_sink && live ? __ldg(p.attn_sink + head) * kLog2e : -INFINITY;
+    float M = many ? -INFINITY : s2, lt = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = r0; r <= r1; ++r) {
-      const float2 ml = a.part_ml[slot(r) * 128 + m];
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;        // the piece holds no key of this row
-      const float w = ex2(ml.x - M);
-      const float4 v = reinterpret_cast<const float4*>(a.part_o)[(slot(r) * (a.dvp / 4) + grp) * 128 + m];
-      lt = fmaf(ml.y, w, lt);
-      o.x = fmaf(v.x, w, o.x);
-      o.y = fmaf(v.y, w, o.y);
-      o.z = fmaf(v.z, w, o.z);
-      o.w = fmaf(v.w, w, o.w);
+    if (live) join_pieces(a, tile, m, grp, r0, many ? r0 + warp : r0, r1, many ? kJoinWarps : 1, M, lt, o);
+    if (many) {
+      __syncthreads();                                        // the item before has been read
+      part_o[warp][lane] = o;
+      part_ml[warp][lane] = make_float2(M, lt);
+      __syncthreads();
+      if (warp != 0) continue;
+      M = s2;
+#pragma unroll 1
+      for (int k = 0; k < kJoinWarps; ++k) M = fmaxf(M, part_ml[k][lane].x);
+      lt = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int k = 0; k < kJoinWarps; ++k) {
+        const float2 ml = part_ml[k][lane];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float w = ex2(ml.x - M);
+        const float4 v = part_o[k][lane];
+        lt = fmaf(ml.y, w, lt);
+        o.x = fmaf(v.x, w, o.x);
+        o.y = fmaf(v.y, w, o.y);
+        o.z = fmaf(v.z, w, o.z);
+        o.w = fmaf(v.w, w, o.w);
+      }
     }
+    if (!live) continue;
+    if (s2 != -INFINITY) lt += ex2(s2 - M);
     const bool none = lt == 0.f;
     const float inv = none ? 0.f : 1.f / lt;
     if (none) o = make_float4(0.f, 0.f, 0.f, 0.f);
-    store4<T>(out + row * p.o_st + (int64_t)head * p.o_sh + grp * 4,
+    store4<T>(static_cast<T*>(p.o) + row * p.o_st + (int64_t)head * p.o_sh + grp * 4,
               make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     if (grp == 0) p.lse[row * p.l_st + (int64_t)head * p.l_sh] = none ? -INFINITY : (M + lg2(lt)) * kLn2;
   }
@@ -273,9 +333,13 @@ static cudaError_t launch(Plan& pl, const CUtensorMap& tq, const CUtensorMap& tk
     if ((e = cudaMemsetAsync(a.cum, 0, ((size_t)a.p.num_seqs + 1) * sizeof(int32_t), st)) != cudaSuccess) return e;
     note_memset("tree_cum", st);
   }
-  const int items = pl.tile_rows * (a.p.d_v / 4);
-  const dim3 grid((unsigned)(a.p.num_seqs * a.p.h_kv * a.ntiles + 1), (unsigned)std::min(8, (items + 255) / 256));
-  tree_combine_kernel<T><<<grid, 256, 0, st>>>(a, pl.tile_rows);
+  // a warp an item of 32 rows; as many CTAs as two per SM where units are few (eight each: 195 us for the
+  // 74 pieces above)
+  const int items = (pl.tile_rows + 31) / 32 * (a.p.d_v / 4);
+  const int units = a.p.num_seqs * a.p.h_kv * a.ntiles, most = std::max(8, 2 * device_sm_count() / std::max(1, units));
+  const int per = a.ranges >= kManyPieces ? 1 : kJoinWarps;   // items of a CTA at a time, where a unit can have many pieces
+  const dim3 grid((unsigned)(units + 1), (unsigned)std::min(most, (items + per - 1) / per));
+  tree_combine_kernel<T><<<grid, kJoinWarps * 32, 0, st>>>(a, pl.tile_rows);
   note_launch("tree_combine", st);
   return cudaGetLastError();
 }
