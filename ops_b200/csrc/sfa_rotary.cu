@@ -274,7 +274,9 @@ struct Steps {
 // L lanes per row, NS units per lane (unit s * L + lane).  The rows of the next steps are on their way
 // into shared memory while one is worked on.  Loaded into registers instead, a step's rows leave nothing
 // in flight while they are worked on: 763 us for norm, rotary and gradients of 4 x 8192 tokens of 64 + 4
-// heads of 128, against 538 us here.  Forward: 3 CTAs per SM (559 us with 2; the backward's registers allow 2).
+// heads of 128, against 525 us here (436 us would be the five passes over q and k at copy rate; instruction
+// issue is 74 % busy in the forward, 62 % in the backward).  Forward: 3 CTAs per SM (20 us more with 2; the
+// backward's registers allow 2).
 // Dynamic shared memory: the ring, the turn steps of the rot / 2 pairs, their (cos, sin) for each warp's token.
 template <typename T, int P, int L, int NS, bool BWD>
 __global__ void __launch_bounds__(kWarps * 32, BWD || NS > 1 ? 2 : 3)
@@ -312,26 +314,39 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
   at.len = p.len;
   at.batch = p.batch;
   Steps ahead = at;
-  bool more = ahead.open(), fresh = true;
+  bool more = ahead.open(), fresh = true, moved = true;
+  const T* ax = nullptr;                                       // the lane's row at `ahead`
+  const T* ady = nullptr;
+  // a lane without a unit reads zeros: nobody copies into its part of the ring
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    if (!has[s])
+#pragma unroll 1
+      for (int i = 0; i < S * (K / NS); ++i)
+        for (int b = 0; b < R; b += 4)
+          *reinterpret_cast<uint32_t*>(ring + ((i / (K / NS)) * K + s * (K / NS) + i % (K / NS)) * kWarps * 32 * R + b) = 0;
   // asks for the rows of the step at `ahead`, into `stage`
   auto ask = [&](int stage) {
     if (more) {
-      const int h = ahead.h + sub;
-      const T* x = static_cast<const T*>(t.x) + ahead.b * t.x_sb + ahead.tt * t.x_st + h * t.x_sh;
-      const T* dy = BWD ? static_cast<const T*>(t.dy) + ahead.b * t.dy_sb + ahead.tt * t.dy_st + h * t.dy_sh : nullptr;
+      if (moved) {
+        ax = static_cast<const T*>(t.x) + ahead.b * t.x_sb + ahead.tt * t.x_st + (ahead.h + sub) * t.x_sh;
+        if (BWD) ady = static_cast<const T*>(t.dy) + ahead.b * t.dy_sb + ahead.tt * t.dy_st + (ahead.h + sub) * t.dy_sh;
+      }
+      const bool row = ahead.h + sub < ahead.h1;
       uint8_t* dst = ring + stage * K * kWarps * 32 * R;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
-        if (h < ahead.h1 && has[s]) {
-          copy_async<R>(dst + (s * (K / NS)) * kWarps * 32 * R, x + un[s].lo);
-          copy_async<R>(dst + (s * (K / NS) + 1) * kWarps * 32 * R, x + un[s].hi);
+        if (row && has[s]) {
+          copy_async<R>(dst + (s * (K / NS)) * kWarps * 32 * R, ax + un[s].lo);
+          copy_async<R>(dst + (s * (K / NS) + 1) * kWarps * 32 * R, ax + un[s].hi);
           if (BWD) {
-            copy_async<R>(dst + (s * (K / NS) + 2) * kWarps * 32 * R, dy + un[s].lo);
-            copy_async<R>(dst + (s * (K / NS) + 3) * kWarps * 32 * R, dy + un[s].hi);
+            copy_async<R>(dst + (s * (K / NS) + 2) * kWarps * 32 * R, ady + un[s].lo);
+            copy_async<R>(dst + (s * (K / NS) + 3) * kWarps * 32 * R, ady + un[s].hi);
           }
         }
-      bool f;
-      more = ahead.next(RPW, f);
+      more = ahead.next(RPW, moved);
+      ax += RPW * t.x_sh;
+      if (BWD) ady += RPW * t.dy_sh;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -415,25 +430,21 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
     uint64_t sq = 0, sd = 0;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const bool on = h < at.h1 && has[s];
+      // rows past the heads are worked on too (what lies in the ring), and not stored
+      Run<T, P> lo, hi;
+      lo.read(src + (s * (K / NS)) * kWarps * 32 * R);
+      hi.read(src + (s * (K / NS) + 1) * kWarps * 32 * R);
+      take<T, P>(lo, hi, inter, va[s], vb[s]);
+      if (BWD) {
+        lo.read(src + (s * (K / NS) + 2) * kWarps * 32 * R);
+        hi.read(src + (s * (K / NS) + 3) * kWarps * 32 * R);
+        take<T, P>(lo, hi, inter, ga[s], gb[s]);
+        if (un[s].pair >= 0) {
 #pragma unroll
-      for (int j = 0; j < H; ++j) va[s][j] = vb[s][j] = ga[s][j] = gb[s][j] = 0;
-      if (on) {
-        Run<T, P> lo, hi;
-        lo.read(src + (s * (K / NS)) * kWarps * 32 * R);
-        hi.read(src + (s * (K / NS) + 1) * kWarps * 32 * R);
-        take<T, P>(lo, hi, inter, va[s], vb[s]);
-        if (BWD) {
-          lo.read(src + (s * (K / NS) + 2) * kWarps * 32 * R);
-          hi.read(src + (s * (K / NS) + 3) * kWarps * 32 * R);
-          take<T, P>(lo, hi, inter, ga[s], gb[s]);
-          if (un[s].pair >= 0) {
-#pragma unroll
-            for (int j = 0; j < H; ++j) {
-              const uint64_t u = fma2(gb[s][j], sn[s][j], mul2(ga[s][j], c[s][j]));
-              gb[s][j] = fma2(neg2(ga[s][j]), sn[s][j], mul2(gb[s][j], c[s][j]));
-              ga[s][j] = u;
-            }
+          for (int j = 0; j < H; ++j) {
+            const uint64_t u = fma2(gb[s][j], sn[s][j], mul2(ga[s][j], c[s][j]));
+            gb[s][j] = fma2(neg2(ga[s][j]), sn[s][j], mul2(gb[s][j], c[s][j]));
+            ga[s][j] = u;
           }
         }
       }
@@ -693,8 +704,8 @@ static Shape shape_of(const SfaRotaryParams& p, bool bwd) {
 // be too few items to fill the SMs (a decode step), down to one step each.
 // The CTAs are shared out by work, an item's cosines counted as four steps: by heads alone, the few CTAs of
 // a lone kv head ran 100 us behind the others.  Two CTAs per SM where each warp has few items (5003 tokens of
-// 10 + 2 heads: 40 us, against 47 with eight), up to eight where that leaves it four (559 against 646 us
-// for 32768 tokens), so that the SMs finish together.
+// 10 + 2 heads: 41 us, against 47 with eight), up to eight where that leaves it four (86 us less than with
+// three for 32768 tokens), so that the SMs finish together.
 static Grid make_grid(const SfaRotaryParams& p, const Shape& s) {
   Grid g{};
   const int sms = device_sm_count(), rpw = s.p ? 32 / s.lanes : 1;
