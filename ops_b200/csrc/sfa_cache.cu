@@ -7,8 +7,12 @@
 //
 // Bookkeeping runs in one CTA (its cost is a few dependent passes over tables of
 // some thousand entries; several CTAs would spend as long on meeting each other);
-// pages and rows are then moved by as many CTAs as fill the SMs, at the rate of
-// HBM, from lists that the bookkeeping left in the workspace.
+// pages and rows are then moved by as many CTAs as fill the SMs, from lists that
+// the bookkeeping left in the workspace.  Measured: 2.35 GB read and written to
+// move some 1100 pages of 128 KB in each of 8 pools in 394 us (0.91 of the measured copy
+// rate); a beam step of 64 sequences (trim 3, fork 9, its 32 pages in 16 pools 19,
+// reserve 8 us); the accepted rows of 128 trees in 32 pools 25 us, where one CTA
+// for each sequence and pool leaves a chain of dependent reads to wait for.
 #include "sfa_common.cuh"
 #include "sfa_internal.h"
 

@@ -1,19 +1,30 @@
 // sfa_tree_pair.cu — the tree attention of sfa_tree.cu with two softmax
 // warpgroups per CTA (d_v <= 128).
 //
-// A warpgroup's work between two MMAs (read S, maximum, exponentials, P back to
-// TMEM) takes about as long as the MMAs and their hand-overs, so two of them take
+// A warpgroup's work between two MMAs (read S, exponentials, P back to TMEM)
+// takes about as long as the MMAs and their hand-overs, so two of them take
 // turns on the tensor core: each has its own S and O in TMEM (2 x 128 + 2 x 128
 // columns) and works on chunks of 128 keys, the width at which the MMAs run at
 // full rate.  What the two share depends on the rows:
 //   rows: two row tiles (256 rows) against the same chunk, which is loaded once
-//         for both: large trees, bound by the exponentials;
+//         for both: large trees, bound by the chain below;
 //   keys: one row tile, alternate chunks; the two (m, l, O) are joined at the end
 //         of the piece out of TMEM: decoding and small trees, bound by reads.
 // A CTA goes by piece: it falls back to `keys` where its second tile is empty.
 //
-// Warps: 0 K, Q and key masks; 1 V; 2 MMA issue (one thread); 3 clears value rows
-// that must not enter a product (see scrub); 4-7 and 8-11 softmax.
+// Measured: one token for each of 16 sequences of 4096 to 32768 keys, 64 heads on
+// 8, 178 us at 5.2 TB/s (0.79 of the measured copy rate); 64-node trees on 8
+// sequences 244 us, 790 TFLOP/s (0.48 of the measured peak).  There a period of
+// 4600 clocks covers 128 keys for both tiles: 2300 from S to P (1024 of them the
+// exponentials' floor) and 2300 from P to the next S (1024 of them MMAs).  Not
+// better: S in halves of 64 keys (half the MMA rate; 251 us), P handed over in
+// halves (266), an issuing warp per warpgroup (281), softmax in steps of 32 keys
+// (280).  The loops are rolled and the MMAs issued from a converged warp because
+// the roles together have to fit the instruction cache: unrolled (148 KB of code)
+// the first case took 408 us.
+//
+// Warps: 0 K, Q and key masks; 1 V; 2 MMA issue; 3 clears value rows that must not
+// enter a product (see scrub); 4-7 and 8-11 softmax.
 // Every wait is bounded (~2 s); on expiry the kernel records (8 << 16) | site in
 // the status word and returns.
 #include "sfa_tree_roles.cuh"
