@@ -41,7 +41,7 @@ def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Op
     bad = len(lead) < 2 or lead[1] < 1 or num_pages not in (None, lead[0])
     values = []
     for t in pools:
-        if bad or t.shape[:2] != lead or t.device != device:
+        if bad or t.device != device or t.shape[:2] != lead:
             raise ValueError("every pool must be [num_pages, page_size, ...] with the same pages, on the device of the table")
         size = t.element_size()
         if t.is_contiguous():

@@ -13,8 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -64,8 +63,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return f.to(device) if device is not None else f, amplitude
 
 
-@dataclass(frozen=True)
-class _Cfg:
+class _Cfg(NamedTuple):
     rot: int
     start: int
     interleaved: bool
@@ -86,10 +84,11 @@ def _strides(x: torch.Tensor):
 def _check(name: str, x: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
     if x.dtype not in _DTYPE:
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() not in (3, 4) or x.shape[-2] < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    if not 3 <= len(shape) <= 4 or shape[-2] < 1 or shape[-1] < 1:
         raise ValueError(f"{name} must be [B, T, H, D] or [T, H, D] with at least one head and dim")
-    if like is not None and (x.dtype != like.dtype or x.device != like.device or x.shape[:-2] != like.shape[:-2]
-                             or x.shape[-1] != like.shape[-1]):
+    if like is not None and (x.dtype != like.dtype or x.device != like.device or shape[:-2] != like.shape[:-2]
+                             or shape[-1] != like.shape[-1]):
         raise ValueError(f"{name} must have q's type, device, tokens and head size")
 
 
@@ -130,7 +129,7 @@ def _weight(name: str, w: Optional[torch.Tensor], x: torch.Tensor) -> Optional[t
         return None
     if w.dim() != 1 or w.shape[0] != x.shape[-1] or w.device != x.device or not w.is_floating_point():
         raise ValueError(f"{name} must be a floating-point vector of the head size on the inputs' device")
-    return w if w.dtype == torch.float32 and w.is_contiguous() else w.float().contiguous()
+    return w if w.dtype is torch.float32 and w.is_contiguous() else w.float().contiguous()
 
 
 _pack = _lib.packer(SfaRotaryParams)
@@ -139,30 +138,34 @@ _NO_TENSOR = (0,) * 20
 _NO_CACHE = (0, 0, 0, 0)
 
 
-def _tensor(x, w, y=None, dy=None, dx=None, dw=None, turned=_TURN):
-    """The values of one SfaRotaryTensor."""
-    return (x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if dy is None else dy.data_ptr(),
-            0 if dx is None else dx.data_ptr(), 0 if w is None else w.data_ptr(), 0 if dw is None else dw.data_ptr(),
-            *_strides(x), *(_strides(y) if y is not None else (0, 0, 0)), *(_strides(dy) if dy is not None else (0, 0, 0)),
-            *(_strides(dx) if dx is not None else (0, 0, 0)), x.shape[-2], turned)
+def _tensor(x, w, y=None, dy=None, dx=None, dw=None):
+    """The values of one SfaRotaryTensor: y forward, dy and dx backward."""
+    head = (x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if dy is None else dy.data_ptr(),
+            0 if dx is None else dx.data_ptr(), 0 if w is None else w.data_ptr(), 0 if dw is None else dw.data_ptr())
+    if y is not None:
+        return head + _strides(x) + _strides(y) + (0, 0, 0, 0, 0, 0, x.shape[-2], _TURN)
+    return head + _strides(x) + (0, 0, 0) + _strides(dy) + _strides(dx) + (x.shape[-2], _TURN)
 
 
-def _paged(x, w, pool, turned):
+def _paged(x, w, pool, stride, turned):
     """The values of one SfaRotaryTensor that goes into a page pool."""
-    return (x.data_ptr(), pool.data_ptr(), 0, 0, 0 if w is None else w.data_ptr(), 0, *_strides(x), 0, pool.stride(1),
-            pool.stride(2), 0, 0, 0, 0, 0, 0, x.shape[-2], turned | _PAGED)
+    xs = x.stride()
+    return (x.data_ptr(), pool.data_ptr(), 0, 0, 0 if w is None else w.data_ptr(), 0, 0, xs[0], xs[1], 0, stride[1],
+            stride[2], 0, 0, 0, 0, 0, 0, x.shape[1], turned | _PAGED)
 
 
 def _params(x: torch.Tensor, tensors, cfg: _Cfg, positions, frequencies, cache=_NO_CACHE, sizes=_NO_CACHE) -> SfaRotaryParams:
-    batch, length = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
+    shape = x.shape
+    batch, length = (shape[0], shape[1]) if len(shape) == 4 else (1, shape[0])
     if positions is None:
         pos, freq, sb, st, p64 = 0, 0, 0, 0, 0
     else:
         pos, freq, p64 = positions.data_ptr(), frequencies.data_ptr(), int(positions.dtype == torch.int64)
-        sb, st = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+        ps = positions.stride()
+        sb, st = ps if len(ps) == 2 else (0, ps[0])
     n = len(tensors)
     return _pack(*tensors[0], *(tensors[1] if n > 1 else _NO_TENSOR), *(tensors[2] if n > 2 else _NO_TENSOR), pos, freq,
-                 *cache, sb, st, n, batch, length, x.shape[-1], cfg.rot, cfg.start, int(cfg.interleaved), _DTYPE[x.dtype],
+                 *cache, sb, st, n, batch, length, shape[-1], cfg.rot, cfg.start, int(cfg.interleaved), _DTYPE[x.dtype],
                  p64, *sizes, cfg.eps, cfg.amplitude, 0)
 
 
@@ -174,9 +177,9 @@ class _NormRotary(torch.autograd.Function):
         if k is not None:
             ok = torch.empty_like(k, memory_format=torch.contiguous_format)
             tensors.append(_tensor(k, wk, ok))
-        P = _params(q, tensors, cfg, positions, frequencies)
-        with _lib.on(q.device):
-            _lib.check(_lib.load().sfa_rotary_fwd(ctypes.byref(P), _lib.stream_of(q.device)), "sfa_rotary_fwd")
+        P, device = _params(q, tensors, cfg, positions, frequencies), q.device
+        with _lib.on(device):
+            _lib.check(_lib.load().sfa_rotary_fwd(ctypes.byref(P), _lib.stream_of(device)), "sfa_rotary_fwd")
         ctx.save_for_backward(q, k, wq, wk, positions, frequencies)
         ctx.cfg = cfg
         return (oq, ok) if k is not None else oq
@@ -243,19 +246,26 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.T
     return _NormRotary.apply(_rows(q), _rows(k), wq, wk, positions, frequencies, cfg)
 
 
-def _check_pool(name: str, c: torch.Tensor, like: torch.Tensor) -> None:
+def _check_pool(name: str, c: torch.Tensor, like: torch.Tensor):
+    """A page pool's shape and strides."""
     if c.dim() != 4 or c.device != like.device:
         raise ValueError(f"{name} must be a [num_pages, page_size, H, D] page pool on the inputs' device")
-    if c.shape[3] > 1 and c.stride(-1) != 1 or c.shape[0] > 1 and c.stride(0) != c.shape[1] * c.stride(1):
+    shape, stride = c.shape, c.stride()
+    pages, page, _, d = shape
+    if d > 1 and stride[3] != 1 or pages > 1 and stride[0] != page * stride[1]:
         raise ValueError(f"{name}: pages must be [page_size, H, D] row ranges of one pool, innermost dim contiguous")
+    return shape, stride
 
 
-def _check_table(block_table: torch.Tensor, cache_seqlens: torch.Tensor, like: torch.Tensor) -> None:
+def _check_table(block_table: torch.Tensor, cache_seqlens: torch.Tensor, like: torch.Tensor):
+    """(sequences, pages of a row of the table)."""
     for name, t, d in (("block_table", block_table, 2), ("cache_seqlens", cache_seqlens, 1)):
         if t.dtype != torch.int32 or t.dim() != d or t.device != like.device:
             raise ValueError(f"{name} must be a {d}-D int32 tensor on the inputs' device")
-    if cache_seqlens.shape[0] != block_table.shape[0]:
+    n, width = block_table.shape
+    if cache_seqlens.shape[0] != n:
         raise ValueError("block_table and cache_seqlens must name the same number of sequences")
+    return n, width
 
 
 def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor],
@@ -279,41 +289,45 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     positions (the depth of a drafted node).  Rows behind the last sequence,
     negative cache positions, positions behind the table and page ids outside
     the pool are not stored.  ``v`` may have another head size than k."""
-    for name, x in (("q", q), ("k", k), ("v", v)):
+    qs, ks, vs, dtype, device = q.shape, k.shape, v.shape, q.dtype, q.device
+    for name, x, shape in (("q", q, qs), ("k", k, ks), ("v", v, vs)):
         _check(name, x)
-        if x.dim() != 3 or x.dtype != q.dtype or x.device != q.device or x.shape[0] != q.shape[0]:
+        if len(shape) != 3 or x.dtype != dtype or x.device != device or shape[0] != qs[0]:
             raise ValueError(f"{name} must be [total, H, D] with q's type, device and rows")
-    if k.shape[-1] != q.shape[-1] or v.shape[1] != k.shape[1]:
+    if ks[2] != qs[2] or vs[1] != ks[1]:
         raise ValueError("k must have q's head size and v must have k's heads")
-    for name, c, x in (("k_cache", k_cache, k), ("v_cache", v_cache, v)):
-        _check_pool(name, c, q)
-        if c.dtype != q.dtype or tuple(c.shape[2:]) != tuple(x.shape[1:]):
+    pools = []
+    for name, c, rows in (("k_cache", k_cache, ks), ("v_cache", v_cache, vs)):
+        pools.append(_check_pool(name, c, q))
+        (_, _, h, d), _ = pools[-1]
+        if c.dtype != dtype or h != rows[1] or d != rows[2]:
             raise ValueError(f"{name} must have the type, heads and head size of the rows stored into it")
-    if v_cache.shape[:2] != k_cache.shape[:2]:
+    (num_pages, page, _, _), kst = pools[0]
+    (v_pages, v_page, _, _), vst = pools[1]
+    if v_pages != num_pages or v_page != page:
         raise ValueError("k_cache and v_cache must have the same pages")
     if k_cache.data_ptr() == v_cache.data_ptr() != 0:
         raise ValueError("k_cache and v_cache must not be the same memory")
-    _check_table(block_table, cache_seqlens, q)
-    n = block_table.shape[0]
+    n, width = _check_table(block_table, cache_seqlens, q)
     if cu_seqlens is None:
-        if q.shape[0] != n:
+        if qs[0] != n:
             raise ValueError("without cu_seqlens, q must hold one row per sequence")
-    elif cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (n + 1,) or cu_seqlens.device != q.device:
+    elif cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (n + 1,) or cu_seqlens.device != device:
         raise ValueError("cu_seqlens must be int32 [n + 1] on the inputs' device")
     cfg, positions, frequencies = _check_turn(q, positions, frequencies, interleaved, start, eps, amplitude)
     wq, wk = _weight("q_weight", q_weight, q), _weight("k_weight", k_weight, k)
     _need_cuda(q)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] < 2 else block_table.contiguous()
+    table = block_table if width < 2 or block_table.stride(1) == 1 else block_table.contiguous()
     lens = cache_seqlens.contiguous()
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     cache = (table.data_ptr(), lens.data_ptr(), 0 if cu is None else cu.data_ptr(), table.stride(0))
-    sizes = (n, k_cache.shape[0], k_cache.shape[1], table.shape[1])
-    tensors = [_tensor(q, wq, out), _paged(k, wk, k_cache, _TURN), _paged(v, None, v_cache, 0)]
-    lib, stream = _lib.load(), _lib.stream_of(q.device)
-    with _lib.on(q.device):
-        if v.shape[-1] != q.shape[-1]:             # v's rows alone: their head size is another
+    sizes = (n, num_pages, page, width)
+    tensors = [_tensor(q, wq, out), _paged(k, wk, k_cache, kst, _TURN), _paged(v, None, v_cache, vst, 0)]
+    lib, stream = _lib.load(), _lib.stream_of(device)
+    with _lib.on(device):
+        if vs[2] != qs[2]:             # v's rows alone: their head size is another
             V = _params(v, tensors[2:], _Cfg(0, 0, False, 0.0, 1.0), None, None, cache, sizes)
             _lib.check(lib.sfa_rotary_fwd(ctypes.byref(V), stream), "sfa_rotary_fwd (append)")
             tensors = tensors[:2]
