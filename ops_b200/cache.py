@@ -109,7 +109,10 @@ def paged_cache_reserve(refcounts: torch.Tensor, block_table: torch.Tensor, cach
     go into the table and ``cache_seqlens`` grows.  Returns ``granted [n]``
     (int32): 1, or 0 where nothing was changed — a negative count, a table too
     narrow, a partly filled last page that other sequences share, or free pages
-    too few for the sequences up to this one together."""
+    too few for the sequences up to this one together.  The new rows of a sequence
+    that was refused must stay out of the calls that follow (``cu_seqlens`` from
+    ``granted * rows``): its length does not include them, so they would be stored
+    over its last ones."""
     _state(refcounts, block_table, cache_seqlens, page_size)
     _ints("add", add, 1, refcounts, block_table.shape[0])
     granted = torch.empty_like(add)

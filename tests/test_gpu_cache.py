@@ -187,7 +187,6 @@ def test_empty_calls():
 def serving_step(state, q, k, v, parents, accepted, cu, m, freq):
     """Room, rows into the pages, attention over them, the accepted path kept."""
     refs, table, lens, kc, vc, page, depth = state
-    n = table.shape[0]
     before = lens.clone()
     granted = ops_b200.paged_cache_reserve(refs, table, lens, torch.full_like(lens, m), page)
     pos = (before[:, None] + depth).view(-1)
@@ -195,7 +194,6 @@ def serving_step(state, q, k, v, parents, accepted, cu, m, freq):
     o, lse = ops_b200.tree_attention_paged(qr, kc, vc, table, lens, parents, cu_seqlens=cu, max_seqlen_q=m)
     keep = ops_b200.paged_cache_accept([kc, vc], table, lens, accepted, torch.full_like(lens, m))
     ops_b200.paged_cache_trim(refs, table, lens, keep, page)
-    del n
     return granted, o, lse
 
 

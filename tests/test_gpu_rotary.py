@@ -247,7 +247,6 @@ def test_append_leaves_out_what_has_no_place():
     # a page of -1, a page id past the pool, a position behind the table, a length below its rows,
     # and rows behind the last sequence: q is still returned for all of them
     hk, D, page = 2, 64, 4
-    counts = [2, 2, 2, 3, 1]
     cu = torch.tensor([0, 2, 4, 6, 9, 10], dtype=torch.int32)
     rows = 13
     q, k, v = make((rows, 4, D), torch.bfloat16, 1), make((rows, hk, D), torch.bfloat16, 2), make((rows, hk, D), torch.bfloat16, 3)
@@ -263,7 +262,45 @@ def test_append_leaves_out_what_has_no_place():
     for row, p, r in ((0, 0, 3), (4, 3, 3), (8, 4, 0), (9, 5, 3)):
         want_k[p, r], want_v[p, r] = k[row], v[row]
     assert torch.equal(gk.cpu(), want_k) and torch.equal(gv.cpu(), want_v)
-    del counts
+
+
+def test_append_past_32_bit_offsets():
+    q, k, v, kc, vc, table, lens, cu, _ = pool_case(3, [2, 1, 5], 8, 8, 128, 128, 64, torch.bfloat16, 15)
+    f, _ = ops_b200.rotary_frequencies(128, device="cuda")
+    pos = torch.arange(8, dtype=torch.int32).cuda()
+    rest = cuda(lens)
+    small = [kc.cuda(), vc.cuda()]
+    want = ops_b200.qk_norm_rotary_append(*cuda(q, k, v), pos, f, *small, table.cuda(), *rest, cu_seqlens=cu.cuda())
+    pages = 2 ** 31 // (64 * 8 * 128) + 2 + kc.shape[0]
+    big = []
+    for c in (kc, vc):
+        big.append(torch.zeros(pages, 64, 8, 128, dtype=torch.bfloat16, device="cuda"))
+        big[-1][-kc.shape[0]:] = c.cuda()
+    got = ops_b200.qk_norm_rotary_append(*cuda(q, k, v), pos, f, *big, (table + pages - kc.shape[0]).cuda(), *rest,
+                                         cu_seqlens=cu.cuda())
+    assert torch.equal(got, want)
+    for b, c in zip(big, small):
+        assert torch.equal(b[-kc.shape[0]:], c) and not b[:-kc.shape[0]].any()
+
+
+def test_rows_past_32_bit_offsets():
+    T = 2 ** 31 // (64 * 128) + 70
+    f, _ = ops_b200.rotary_frequencies(128, device="cuda")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    w = torch.rand(128, device="cuda")
+    x = torch.zeros(T, 64, 128, dtype=torch.bfloat16, device="cuda")
+    x[-64:] = make((64, 64, 128), torch.bfloat16, 4).cuda()
+    x[-64:].mul_(2)
+    x.requires_grad_()
+    y, _ = ops_b200.qk_norm_rotary(x, x[:, :1], pos, f, w)
+    tail = x.detach()[-64:].clone().requires_grad_()
+    want, _ = ops_b200.qk_norm_rotary(tail, tail[:, :1], pos[-64:], f, w)
+    assert torch.equal(y[-64:], want) and not y[:-64].any()
+    dy = torch.zeros_like(y)
+    dy[-64:] = make((64, 64, 128), torch.bfloat16, 5).cuda()
+    dx, = torch.autograd.grad(y, x, dy)
+    want, = torch.autograd.grad(want, tail, dy[-64:])
+    assert torch.equal(dx[-64:], want) and not dx[:-64].any()
 
 
 def test_append_on_another_stream_and_in_a_graph():
