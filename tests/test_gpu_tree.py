@@ -131,12 +131,17 @@ def test_defaults_scale_and_strides():
     check(got, ref, q, vc, 201)
 
 
+KINDS = pytest.mark.parametrize("hq,dqk,dv", [(8, 64, 72), (64, 64, 72), (8, 128, 200), (64, 256, 136)],
+                                ids=["one tile", "several tiles", "wide", "wide, several tiles"])
+
+
+@KINDS
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("where", ["first chunk", "later chunk"])
-def test_what_a_row_does_not_see_does_not_matter(dtype, where):
+def test_what_a_row_does_not_see_does_not_matter(dtype, where, hq, dqk, dv):
     # a drafted row's NaN and infinite keys and values reach its descendants and nobody else
     prefix = 3 if where == "first chunk" else 150
-    q, kc, vc, table, lens, par, cu = problem([9, 4], [prefix, 40], 8, 2, 64, 72, 16, dtype, 5)
+    q, kc, vc, table, lens, par, cu = problem([9, 4], [prefix, 40], hq, 2, dqk, dv, 16, dtype, 5)
     par[:9] = torch.tensor([-1, 0, 0, 1, 1, 2, 4, 5, -1])
 
     def place(j):
@@ -158,10 +163,11 @@ def test_what_a_row_does_not_see_does_not_matter(dtype, where):
     assert torch.isfinite(got[0].cpu()[[0, 1, 4, 6, 9, 10, 11, 12]]).all()
 
 
-def test_missing_pages_short_caches_and_rows_behind():
+@pytest.mark.parametrize("dv", [64, 176])
+def test_missing_pages_short_caches_and_rows_behind(dv):
     # entries outside the pool, a table shorter than the cache, a cache shorter than its drafted rows, no cache,
     # rows behind the last sequence
-    q, kc, vc, table, lens, par, cu = problem([3, 2, 4, 2, 1], [90, 70, 0, 30, 50], 8, 2, 64, 64, 16, torch.bfloat16, 9, behind=5)
+    q, kc, vc, table, lens, par, cu = problem([3, 2, 4, 2, 1], [90, 70, 0, 30, 50], 8, 2, 64, dv, 16, torch.bfloat16, 9, behind=5)
     table[0, 1], table[0, 4], table[1, 2] = -7, kc.shape[0], 2 ** 31 - 1
     table[4, :] = -1                                       # every page of a sequence missing
     lens[2], lens[3] = 2, 0                                # four rows in a cache of two; no cache at all
@@ -175,7 +181,7 @@ def test_missing_pages_short_caches_and_rows_behind():
     none = ops_b200.tree_attention_paged(q.cuda()[:2], kc.cuda()[:0], vc.cuda()[:0], table.cuda()[:2, :0], lens.cuda()[:2])
     assert not none[0].any() and torch.isinf(none[1]).all()
     empty = ops_b200.tree_attention_paged(q.cuda()[:0], kc.cuda(), vc.cuda(), table.cuda()[:0], lens.cuda()[:0])
-    assert empty[0].shape == (0, 8, 64)
+    assert empty[0].shape == (0, 8, dv)
 
 
 def test_rows_before_the_first_sequence_and_bad_offsets():
@@ -216,19 +222,21 @@ def test_pools_past_32_bit_offsets():
     assert torch.equal(got[0].nan_to_num(nan=7.0), want[0].nan_to_num(nan=7.0)) and torch.equal(got[1], want[1])
 
 
-def test_extreme_scores():
+@KINDS
+def test_extreme_scores(hq, dqk, dv):
     # scores that rise by far more than a rescale allows from chunk to chunk, and fall; one key that takes all
-    q, kc, vc, table, lens, par, cu = problem([4, 1], [700, 300], 8, 2, 64, 64, 64, torch.bfloat16, 4, fill=0.0)
+    q, kc, vc, table, lens, par, cu = problem([14, 1], [700, 300], hq, 2, dqk, dv, 64, torch.bfloat16, 4, fill=0.0)
     for t in range(int(lens[0])):
         kc[int(table[0, t // 64]), t % 64] *= (t // 64 + 1) * 2.0
     for t in range(int(lens[1])):
         kc[int(table[1, t // 64]), t % 64] *= 12.0 / (t // 64 + 1)
-    check(run(q, kc, vc, table, lens, par, cu), O.tree_attention(q, kc, vc, table, lens, par, cu_seqlens=cu), q, vc, 704)
+    check(run(q, kc, vc, table, lens, par, cu), O.tree_attention(q, kc, vc, table, lens, par, cu_seqlens=cu), q, vc, 714)
 
 
-def test_streams_graphs_and_repeats():
-    a = problem([16, 3, 1], [900, 10, 64], 16, 2, 128, 128, 64, torch.bfloat16, 2)
-    b = problem([2] * 6, [50] * 6, 16, 2, 128, 128, 64, torch.bfloat16, 6)
+@pytest.mark.parametrize("dv", [128, 192])
+def test_streams_graphs_and_repeats(dv):
+    a = problem([16, 3, 1], [900, 10, 64], 16, 2, 128, dv, 64, torch.bfloat16, 2)
+    b = problem([2] * 6, [50] * 6, 16, 2, 128, dv, 64, torch.bfloat16, 6)
     dev = [[None if t is None else t.cuda() for t in x] for x in (a, b)]
 
     def call(x):
