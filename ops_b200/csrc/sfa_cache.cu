@@ -10,9 +10,9 @@
 // pages and rows are then moved by as many CTAs as fill the SMs, from lists that
 // the bookkeeping left in the workspace.  Measured: 2.35 GB read and written to
 // move some 1100 pages of 128 KB in each of 8 pools in 394 us (0.91 of the measured copy
-// rate); a beam step of 64 sequences (trim 3, fork 9, its 32 pages in 16 pools 19,
-// reserve 8 us); the accepted rows of 128 trees in 32 pools 25 us, where one CTA
-// for each sequence and pool leaves a chain of dependent reads to wait for.
+// rate); a beam step of 64 sequences (trim, fork, its 32 pages in 16 pools, reserve) in
+// 35 us, 20.5 of them the pages' floor; acceptance and trim of 128 trees in 32 pools in
+// 20 us, a chain of dependent reads (lengths, path, table, rows) around 10 us of rows.
 #include "sfa_common.cuh"
 #include "sfa_internal.h"
 
@@ -79,13 +79,15 @@ __device__ __forceinline__ N block_scan(N v, N* total) {
   __syncthreads();
   if (lane == 31) part[warp] = run;
   __syncthreads();
-  N before = 0, all = 0;
-  for (int i = 0; i < kPlan / 32; ++i) {
-    if (i < warp) before += part[i];
-    all += part[i];
+  N sums = part[lane];                                        // each warp scans the warps' sums for itself
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const N up = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += up;
   }
-  *total = all;
-  return before + run - v;
+  *total = __shfl_sync(0xffffffffu, sums, 31);
+  const N before = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
+  return (warp > 0 ? before : 0) + run - v;
 }
 
 // This thread's part of [0, n), the parts ascending with the thread.
@@ -336,28 +338,34 @@ __global__ void __launch_bounds__(kMove) move_kernel(const __grid_constant__ Sfa
   }
 }
 
+struct Rows {              // of one sequence, taken together: -1: stays where it is
+  int page_from[kRows], row_from[kRows], page_to[kRows], row_to[kRows];
+};
+
 // Accepted rows i of a sequence: cache row prefix + a[i] to prefix + i.  A thread owns the same bytes of
 // every row and takes the rows in order; a[i] >= i, so a row is read before a later one is written over it,
 // eight at a time.
 template <typename V>
-__device__ __forceinline__ void move_rows(const SfaCachePool& t, const int64_t* from, const int64_t* to, int n, int64_t row_bytes) {
+__device__ __forceinline__ void move_rows(const SfaCachePool& t, const Rows& r, int n, int64_t row_bytes, int lane, int lanes) {
   char* base = static_cast<char*>(t.base);
-  for (int64_t u = threadIdx.x * sizeof(V); u < row_bytes; u += kMove * sizeof(V))
+  for (int64_t u = lane * sizeof(V); u < row_bytes; u += lanes * sizeof(V))
     for (int i = 0; i < n; i += 8) {
       V v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (i + k < n && from[i + k] >= 0) v[k] = *reinterpret_cast<const V*>(base + from[i + k] + u);
+        if (i + k < n && r.page_from[i + k] >= 0)
+          v[k] = *reinterpret_cast<const V*>(base + r.page_from[i + k] * t.page_stride + r.row_from[i + k] * row_bytes + u);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (i + k < n && from[i + k] >= 0) *reinterpret_cast<V*>(base + to[i + k] + u) = v[k];
+        if (i + k < n && r.page_from[i + k] >= 0)
+          *reinterpret_cast<V*>(base + r.page_to[i + k] * t.page_stride + r.row_to[i + k] * row_bytes + u) = v[k];
     }
 }
 
+// A CTA finds the rows of its sequence once and moves them in several pools, `lanes` threads a pool.
 __global__ void __launch_bounds__(kMove) accept_kernel(const __grid_constant__ SfaCacheParams p, const __grid_constant__ Pools pools,
-                                                       int first_launch) {
-  __shared__ int64_t from[kRows], to[kRows];
-  __shared__ int page_from[kRows], row_from[kRows], page_to[kRows], row_to[kRows];
+                                                       int lanes, int first_launch) {
+  __shared__ Rows rows;
   __shared__ int bad_at;
   const int s = blockIdx.x;
   const int len = p.cache_seqlens[s], m = p.b[s];
@@ -374,41 +382,34 @@ __global__ void __launch_bounds__(kMove) accept_kernel(const __grid_constant__ S
       const int a = acc[i], before = i > 0 ? acc[i - 1] : -1;
       const bool ok = a >= 0 && a < m && a > before;
       if (!ok) atomicMin(&bad_at, (int)threadIdx.x);
-      page_from[threadIdx.x] = page_to[threadIdx.x] = -1;
+      rows.page_from[threadIdx.x] = -1;
       if (ok && a != i) {
         const int x = prefix + a, y = prefix + i;
         const int cx = x / p.page_size, cy = y / p.page_size;
         if (cx < p.table_width && cy < p.table_width) {
           const int px = p.block_table[s * p.bt_stride + cx], py = p.block_table[s * p.bt_stride + cy];
           if (px >= 0 && px < p.num_pages && py >= 0 && py < p.num_pages) {
-            page_from[threadIdx.x] = px;
-            row_from[threadIdx.x] = x % p.page_size;
-            page_to[threadIdx.x] = py;
-            row_to[threadIdx.x] = y % p.page_size;
+            rows.page_from[threadIdx.x] = px;
+            rows.row_from[threadIdx.x] = x % p.page_size;
+            rows.page_to[threadIdx.x] = py;
+            rows.row_to[threadIdx.x] = y % p.page_size;
           }
         }
       }
     }
     __syncthreads();
-    const int take = bad_at;
+    const int take = bad_at, together = kMove / lanes;
     more = take == n;
     kept += take;
-    for (int q = blockIdx.y; q < p.num_pools; q += gridDim.y) {
-      const SfaCachePool t = pools.t[q];
+    for (int q = blockIdx.y * together + threadIdx.x / lanes; q < p.num_pools; q += gridDim.y * together) {
+      const SfaCachePool& t = pools.t[q];
       const int64_t row_bytes = t.page_bytes / p.page_size;
-      if (threadIdx.x < take) {
-        const int px = page_from[threadIdx.x];
-        from[threadIdx.x] = px < 0 ? -1 : px * t.page_stride + row_from[threadIdx.x] * row_bytes;
-        to[threadIdx.x] = px < 0 ? -1 : page_to[threadIdx.x] * t.page_stride + row_to[threadIdx.x] * row_bytes;
-      }
-      __syncthreads();
-      const int unit = unit_of(t, row_bytes);
-      if (unit == 16) move_rows<uint4>(t, from, to, take, row_bytes);
-      else if (unit == 4) move_rows<uint32_t>(t, from, to, take, row_bytes);
-      else move_rows<uint8_t>(t, from, to, take, row_bytes);
-      __syncthreads();
+      const int unit = unit_of(t, row_bytes), lane = threadIdx.x % lanes;
+      if (unit == 16) move_rows<uint4>(t, rows, take, row_bytes, lane, lanes);
+      else if (unit == 4) move_rows<uint32_t>(t, rows, take, row_bytes, lane, lanes);
+      else move_rows<uint8_t>(t, rows, take, row_bytes, lane, lanes);
     }
-    __syncthreads();
+    __syncthreads();                                          // the rows have been read
   }
   if (first_launch && blockIdx.y == 0 && threadIdx.x == 0) p.out[s] = fine ? prefix + kept : -1;
 }
@@ -529,7 +530,15 @@ int sfa_cache_accept(const SfaCacheParams* p, void* stream) {
   if (rc || p->num_seqs == 0) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   by_pools(*p, true, [&](const SfaCacheParams& q, const Pools& t, int first) {
-    accept_kernel<<<dim3(q.num_seqs, std::max(1, q.num_pools)), kMove, 0, st>>>(q, t, first);
+    // threads a pool: as many as the widest row has units; CTAs: one wave of eight per SM, each with
+    // several pools (with a CTA for each sequence and pool, acceptance and trim of 128 sequences in 32 pools
+    // took 31 us instead of 20)
+    int lanes = 32;
+    for (int k = 0; k < q.num_pools; ++k)
+      while (lanes < kMove && t.t[k].page_bytes / q.page_size > 16 * (int64_t)lanes) lanes *= 2;
+    const int most = std::max(1, (q.num_pools + kMove / lanes - 1) / (kMove / lanes));
+    const int y = std::min(most, std::max(1, device_sm_count() * 8 / q.num_seqs));
+    accept_kernel<<<dim3(q.num_seqs, y), kMove, 0, st>>>(q, t, lanes, first);
     note_launch("cache_accept", st);
   });
   return done("accept");
