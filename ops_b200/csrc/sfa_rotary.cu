@@ -278,7 +278,7 @@ struct Steps {
 // issue is 74 % busy in the forward, 62 % in the backward).  Forward: 3 CTAs per SM (20 us more with 2; the
 // backward's registers allow 2).
 // Dynamic shared memory: the ring, the turn steps of the rot / 2 pairs, their (cos, sin) for each warp's token.
-template <typename T, int P, int L, int NS, bool BWD>
+template <typename T, int P, int L, int NS, bool BWD, bool INTER>
 __global__ void __launch_bounds__(kWarps * 32, BWD || NS > 1 ? 2 : 3)
 rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__ Grid g) {
   constexpr int RPW = 32 / L, H = P / 2, R = P * (int)sizeof(T), S = stages<NS>(), K = NS * (BWD ? 4 : 2);
@@ -291,7 +291,8 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
   int ti = 0, cta = blockIdx.x;
   while (cta >= g.ctas[ti]) cta -= g.ctas[ti++];
   const SfaRotaryTensor& t = p.t[ti];
-  const bool turned = (t.flags & SFA_ROTARY_TURN) && p.rot > 0, inter = p.interleaved != 0;
+  const bool turned = (t.flags & SFA_ROTARY_TURN) && p.rot > 0;
+  constexpr bool inter = INTER;
   const bool norm = t.weight != nullptr;
   const bool paged = !BWD && (t.flags & SFA_ROTARY_PAGED);
   const int units = p.dim / (2 * P);
@@ -739,13 +740,19 @@ static int total_ctas(const SfaRotaryParams& p, const Grid& g) {
   return n;
 }
 
-template <typename T, int P, int L, int NS, bool BWD>
-static void launch_shape(const SfaRotaryParams& p, const Grid& g, cudaStream_t st) {
+template <typename T, int P, int L, int NS, bool BWD, bool INTER>
+static void launch_layout(const SfaRotaryParams& p, const Grid& g, cudaStream_t st) {
   const size_t turns = (size_t)(p.rot / 2) * (sizeof(uint64_t) + kWarps * sizeof(float2));   // at most 36 KB
   const size_t smem = std::max(ring_bytes<T, P, NS, BWD>() + turns, BWD ? kWarps * sizeof(float) * p.dim : (size_t)0);
   if (smem > 48 * 1024)
-    cudaFuncSetAttribute(rotary_kernel<T, P, L, NS, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  rotary_kernel<T, P, L, NS, BWD><<<total_ctas(p, g), kWarps * 32, smem, st>>>(p, g);
+    cudaFuncSetAttribute(rotary_kernel<T, P, L, NS, BWD, INTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  rotary_kernel<T, P, L, NS, BWD, INTER><<<total_ctas(p, g), kWarps * 32, smem, st>>>(p, g);
+}
+
+template <typename T, int P, int L, int NS, bool BWD>
+static void launch_shape(const SfaRotaryParams& p, const Grid& g, cudaStream_t st) {
+  if (p.interleaved) launch_layout<T, P, L, NS, BWD, true>(p, g, st);
+  else launch_layout<T, P, L, NS, BWD, false>(p, g, st);
 }
 
 template <typename T, int P, bool BWD>
