@@ -274,7 +274,7 @@ struct Steps {
 // L lanes per row, NS units per lane (unit s * L + lane).  The rows of the next steps are on their way
 // into shared memory while one is worked on.  Loaded into registers instead, a step's rows leave nothing
 // in flight while they are worked on: 763 us for norm, rotary and gradients of 4 x 8192 tokens of 64 + 4
-// heads of 128, against 525 us here (436 us would be the five passes over q and k at copy rate; instruction
+// heads of 128, against 507 us here (436 us would be the five passes over q and k at copy rate; instruction
 // issue is 74 % busy in the forward, 62 % in the backward).  Forward: 3 CTAs per SM (20 us more with 2; the
 // backward's registers allow 2).
 // Dynamic shared memory: the ring, the turn steps of the rot / 2 pairs, their (cos, sin) for each warp's token.
