@@ -368,7 +368,7 @@ int sfa_rotary_bwd(const SfaRotaryParams* p, void* workspace, size_t workspace_b
  * rows that no row of the sequence sees do not matter, NaN included, and a row
  * is not touched by what a drafted row it does not see holds.  attn_sink adds
  * exp(sink) to the denominator.  A row that sees nothing gives o = 0 and lse =
- * -inf (or its sink); so do rows behind cu_seqlens[num_seqs].
+ * -inf (or its sink); so do rows outside all sequences and rows past max_q.
  * Types: bf16 or fp16 (dtype), lse fp32; d_qk and d_v multiples of 8 up to 256;
  * strides in elements, multiples of 8, bases 16-byte aligned; scale > 0. */
 #define SFA_TREE_MAX_NODES 256
