@@ -40,7 +40,14 @@ def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Op
     lead, device = pools[0].shape[:2], like.device
     bad = len(lead) < 2 or lead[1] < 1 or num_pages not in (None, lead[0])
     values = []
+    first, same = pools[0], None                       # same: page bytes of contiguous pools like the first
+    if not bad and first.is_contiguous():
+        shape, dtype = first.shape, first.dtype
+        same = first.numel() // max(lead[0], 1) * first.element_size()
     for t in pools:
+        if same is not None and t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous():
+            values += (t.data_ptr(), same, same)
+            continue
         if bad or t.device != device or t.shape[:2] != lead:
             raise ValueError("every pool must be [num_pages, page_size, ...] with the same pages, on the device of the table")
         size = t.element_size()
