@@ -299,9 +299,11 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     pools = []
     for name, c, rows in (("k_cache", k_cache, ks), ("v_cache", v_cache, vs)):
         pools.append(_check_pool(name, c, q))
-        (_, _, h, d), _ = pools[-1]
+        (n, m, h, d), (_, st, sh, _) = pools[-1]
         if c.dtype != dtype or h != rows[1] or d != rows[2]:
             raise ValueError(f"{name} must have the type, heads and head size of the rows stored into it")
+        if n * m > 1 and st < d or h > 1 and sh < d:
+            raise ValueError(f"{name}: rows and heads must not overlap, they are stored into")
     (num_pages, page, _, _), kst = pools[0]
     (v_pages, v_page, _, _), vst = pools[1]
     if v_pages != num_pages or v_page != page:

@@ -98,6 +98,8 @@ def append_args():
     (dict(), "CUDA"), (dict(v=torch.zeros(2, 2, 64)), "v must be"), (dict(v=torch.zeros(3, 1, 64)), "k's heads"),
     (dict(k_cache=torch.zeros(5, 8, 2, 64).half()), "k_cache"), (dict(v_cache=torch.zeros(5, 8, 2, 32)), "v_cache"),
     (dict(v_cache=torch.zeros(4, 8, 2, 64)), "same pages"), (dict(k_cache=ONE_POOL, v_cache=ONE_POOL), "same memory"),
+    (dict(v_cache=torch.zeros(5, 8, 1, 64).expand(5, 8, 2, 64)), "overlap"),
+    (dict(k_cache=torch.zeros(1, 1, 2, 64).expand(5, 8, 2, 64)), "overlap"),
     (dict(k_cache=torch.zeros(5, 2, 8, 64).transpose(1, 2)), "row ranges"),
     (dict(block_table=torch.zeros(3, 2)), "int32"), (dict(cache_seqlens=torch.ones(2, dtype=torch.int32)), "same number"),
     (dict(block_table=torch.zeros(2, 2, dtype=torch.int32), cache_seqlens=torch.ones(2, dtype=torch.int32)), "one row"),
