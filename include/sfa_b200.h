@@ -427,7 +427,11 @@ int sfa_tree_attention(const SfaTreeParams* p, void* workspace, size_t workspace
  *    ascending, ended by -1 or the width; b = [num_seqs] drafted rows.  The
  *    accepted cache rows are moved together behind the prefix, cache_seqlens -
  *    b; out[s] = rows to keep (for trim), -1 for a sequence with b outside
- *    [0, cache_seqlens];
+ *    [0, cache_seqlens], or one whose rows would be moved into a page with a
+ *    reference count above 1: nothing of it moves.  Without refcounts the caller
+ *    answers for it that those pages are the sequence's alone;
+ *  - accept_table: the same with counts of its own.  refcounts is scratch, which
+ *    gets the number of entries of this table that hold each page;
  *  - compact: pages in use are moved to the lowest numbers, refcounts and table
  *    follow; out[0] = pages in use;
  *  - copy: page a[i] to page b[i], i < count.  out[i] = 1 if copied, 0 for a
@@ -456,6 +460,7 @@ int sfa_cache_reserve(const SfaCacheParams* p, void* workspace, size_t workspace
 int sfa_cache_trim(const SfaCacheParams* p, void* stream);
 int sfa_cache_fork(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
 int sfa_cache_accept(const SfaCacheParams* p, void* stream);
+int sfa_cache_accept_table(const SfaCacheParams* p, void* stream);
 int sfa_cache_compact(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
 int sfa_cache_copy(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream);
 

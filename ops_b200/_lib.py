@@ -150,6 +150,7 @@ EXPORTS = {
     "sfa_cache_trim": ([ctypes.POINTER(SfaCacheParams), _c_void_p], _i32),
     "sfa_cache_fork": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_cache_accept": ([ctypes.POINTER(SfaCacheParams), _c_void_p], _i32),
+    "sfa_cache_accept_table": ([ctypes.POINTER(SfaCacheParams), _c_void_p], _i32),
     "sfa_cache_compact": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_cache_copy": ([ctypes.POINTER(SfaCacheParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),
     "sfa_indexer_topk": ([ctypes.POINTER(SfaIndexerParams), _c_void_p, ctypes.c_size_t, _c_void_p], _i32),

@@ -146,7 +146,9 @@ def paged_cache_fork(refcounts: torch.Tensor, block_table: torch.Tensor, cache_s
     page in every pool.  Returns ``forked [f]`` (int32): 1, or 0 where nothing was
     changed — a number outside the table, a target that still holds rows or that
     an earlier fork of the call names, a last page outside the pool, or no free
-    page.  Sources are taken as they were before the call, and may repeat."""
+    page.  Sources are taken as they were before the call, and may repeat.  Rows
+    that were reserved but not stored yet are part of a source's whole pages: store
+    them before the fork, or both sequences would store into one page."""
     _state(refcounts, block_table, cache_seqlens)
     _ints("src", src, 1, refcounts)
     _ints("dst", dst, 1, refcounts, src.shape[0])
@@ -158,23 +160,33 @@ def paged_cache_fork(refcounts: torch.Tensor, block_table: torch.Tensor, cache_s
 
 
 def paged_cache_accept(pools: Sequence[torch.Tensor], block_table: torch.Tensor, cache_seqlens: torch.Tensor,
-                       accepted: torch.Tensor, drafted: torch.Tensor) -> torch.Tensor:
+                       accepted: torch.Tensor, drafted: torch.Tensor, refcounts: Optional[torch.Tensor] = None) -> torch.Tensor:
     """After the verification of drafted trees: of the last ``drafted [n]`` rows of
     each sequence, those named by ``accepted [n, m]`` (int32: ascending row
     numbers of the tree, ended by -1 or the width; an entry that is not above the
     one before or not below ``drafted`` ends it too) are moved together behind
     the prefix, in every pool.  Returns ``keep [n]`` (int32), the rows that each
-    sequence should keep, for ``paged_cache_trim``; -1 where ``drafted`` is
-    negative or above the length."""
+    sequence should keep, for ``paged_cache_trim``; -1 where nothing was moved:
+    ``drafted`` is negative or above the length, or a row would go into a page
+    that another sequence holds too (a fork after the drafted rows were stored
+    shares their whole pages: free one of the two, or fork after the
+    acceptance).  ``refcounts [num_pages]`` says which pages are shared; without
+    it the entries of this table are counted, in a launch of its own, and pages
+    that only another table holds count as unshared."""
     _ints("block_table", block_table, 2, block_table)
     _ints("cache_seqlens", cache_seqlens, 1, block_table, block_table.shape[0])
     _ints("accepted", accepted, 2, block_table, block_table.shape[0])
     _ints("drafted", drafted, 1, block_table, block_table.shape[0])
     arr, num_pages, page = _pool_array(pools, block_table, None)
+    name = "sfa_cache_accept"
+    if refcounts is not None:
+        _ints("refcounts", refcounts, 1, block_table, num_pages)
+    else:
+        name, refcounts = "sfa_cache_accept_table", block_table.new_empty(num_pages)
     keep = torch.empty_like(cache_seqlens)
-    P = _params(None, block_table, cache_seqlens, page, num_pages, accepted if accepted.numel() else drafted, drafted, keep,
+    P = _params(refcounts, block_table, cache_seqlens, page, num_pages, accepted if accepted.numel() else drafted, drafted, keep,
                 arr, accepted.shape[1])
-    _call("sfa_cache_accept", P, block_table, workspace=False)
+    _call(name, P, block_table, workspace=False)
     return keep
 
 

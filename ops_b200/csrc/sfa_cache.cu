@@ -363,6 +363,8 @@ __device__ __forceinline__ void move_rows(const SfaCachePool& t, const Rows& r, 
 }
 
 // A CTA finds the rows of its sequence once and moves them in several pools, `lanes` threads a pool.
+// Nothing of a sequence moves if one of its rows would go into a page that others hold (a fork shares whole
+// pages, those of drafted rows too): a path of several lists is looked through for that first.
 __global__ void __launch_bounds__(kMove) accept_kernel(const __grid_constant__ SfaCacheParams p, const __grid_constant__ Pools pools,
                                                        int lanes, int first_launch) {
   __shared__ Rows rows;
@@ -372,46 +374,64 @@ __global__ void __launch_bounds__(kMove) accept_kernel(const __grid_constant__ S
   const bool fine = m >= 0 && m <= len;
   const int prefix = len - m;
   int kept = 0;
-  bool more = fine;
-  for (int i0 = 0; i0 < p.count && more; i0 += kRows) {
-    const int i = i0 + threadIdx.x, n = min(kRows, p.count - i0);
-    if (threadIdx.x == 0) bad_at = n;
-    __syncthreads();
-    if (threadIdx.x < n) {
-      const int32_t* acc = p.a + s * p.a_stride;
-      const int a = acc[i], before = i > 0 ? acc[i - 1] : -1;
-      const bool ok = a >= 0 && a < m && a > before;
-      if (!ok) atomicMin(&bad_at, (int)threadIdx.x);
-      rows.page_from[threadIdx.x] = -1;
-      if (ok && a != i) {
-        const int x = prefix + a, y = prefix + i;
-        const int cx = x / p.page_size, cy = y / p.page_size;
-        if (cx < p.table_width && cy < p.table_width) {
-          const int px = p.block_table[s * p.bt_stride + cx], py = p.block_table[s * p.bt_stride + cy];
-          if (px >= 0 && px < p.num_pages && py >= 0 && py < p.num_pages) {
-            rows.page_from[threadIdx.x] = px;
-            rows.row_from[threadIdx.x] = x % p.page_size;
-            rows.page_to[threadIdx.x] = py;
-            rows.row_to[threadIdx.x] = y % p.page_size;
+  bool shared = false;
+  for (int pass = p.refcounts && p.count > kRows ? 0 : 1; pass < 2 && !shared; ++pass) {
+    bool more = fine;
+    kept = 0;
+    for (int i0 = 0; i0 < p.count && more; i0 += kRows) {
+      const int i = i0 + threadIdx.x, n = min(kRows, p.count - i0);
+      bool held = false;                                      // by another sequence too: the page this row goes to
+      if (threadIdx.x == 0) bad_at = n;
+      __syncthreads();
+      if (threadIdx.x < n) {
+        const int32_t* acc = p.a + s * p.a_stride;
+        const int a = acc[i], before = i > 0 ? acc[i - 1] : -1;
+        const bool ok = a >= 0 && a < m && a > before;
+        if (!ok) atomicMin(&bad_at, (int)threadIdx.x);
+        rows.page_from[threadIdx.x] = -1;
+        if (ok && a != i) {
+          const int x = prefix + a, y = prefix + i;
+          const int cx = x / p.page_size, cy = y / p.page_size;
+          if (cx < p.table_width && cy < p.table_width) {
+            const int px = p.block_table[s * p.bt_stride + cx], py = p.block_table[s * p.bt_stride + cy];
+            if (px >= 0 && px < p.num_pages && py >= 0 && py < p.num_pages) {
+              held = p.refcounts && p.refcounts[py] > 1;
+              rows.page_from[threadIdx.x] = px;
+              rows.row_from[threadIdx.x] = x % p.page_size;
+              rows.page_to[threadIdx.x] = py;
+              rows.row_to[threadIdx.x] = y % p.page_size;
+            }
           }
         }
       }
+      __syncthreads();
+      const int take = bad_at, together = kMove / lanes;
+      shared = __syncthreads_or(held && (int)threadIdx.x < take);
+      if (shared) break;
+      more = take == n;
+      kept += take;
+      if (pass == 1)
+        for (int q = blockIdx.y * together + threadIdx.x / lanes; q < p.num_pools; q += gridDim.y * together) {
+          const SfaCachePool& t = pools.t[q];
+          const int64_t row_bytes = t.page_bytes / p.page_size;
+          const int unit = unit_of(t, row_bytes), lane = threadIdx.x % lanes;
+          if (unit == 16) move_rows<uint4>(t, rows, take, row_bytes, lane, lanes);
+          else if (unit == 4) move_rows<uint32_t>(t, rows, take, row_bytes, lane, lanes);
+          else move_rows<uint8_t>(t, rows, take, row_bytes, lane, lanes);
+        }
+      __syncthreads();                                        // the rows have been read
     }
-    __syncthreads();
-    const int take = bad_at, together = kMove / lanes;
-    more = take == n;
-    kept += take;
-    for (int q = blockIdx.y * together + threadIdx.x / lanes; q < p.num_pools; q += gridDim.y * together) {
-      const SfaCachePool& t = pools.t[q];
-      const int64_t row_bytes = t.page_bytes / p.page_size;
-      const int unit = unit_of(t, row_bytes), lane = threadIdx.x % lanes;
-      if (unit == 16) move_rows<uint4>(t, rows, take, row_bytes, lane, lanes);
-      else if (unit == 4) move_rows<uint32_t>(t, rows, take, row_bytes, lane, lanes);
-      else move_rows<uint8_t>(t, rows, take, row_bytes, lane, lanes);
-    }
-    __syncthreads();                                          // the rows have been read
   }
-  if (first_launch && blockIdx.y == 0 && threadIdx.x == 0) p.out[s] = fine ? prefix + kept : -1;
+  if (first_launch && blockIdx.y == 0 && threadIdx.x == 0) p.out[s] = fine && !shared ? prefix + kept : -1;
+}
+
+// How many entries of the table hold each page, into refcounts (zeroed before), a CTA a sequence.
+__global__ void __launch_bounds__(kMove) count_kernel(const __grid_constant__ SfaCacheParams p) {
+  const int s = blockIdx.x, n = min(p.table_width, pages_of(p.cache_seqlens[s], p.page_size));
+  for (int c = threadIdx.x; c < n; c += kMove) {
+    const int pg = p.block_table[s * p.bt_stride + c];
+    if (pg >= 0 && pg < p.num_pages) atomicAdd(p.refcounts + pg, 1);
+  }
 }
 
 static int bad(const char* what, const std::string& m) {
@@ -542,6 +562,20 @@ int sfa_cache_accept(const SfaCacheParams* p, void* stream) {
     note_launch("cache_accept", st);
   });
   return done("accept");
+}
+
+int sfa_cache_accept_table(const SfaCacheParams* p, void* stream) {
+  const int rc = check(p, "accept", true, true, true, true, true);
+  if (rc || p->num_seqs == 0) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p->num_pages > 0) {
+    const cudaError_t e = cudaMemsetAsync(p->refcounts, 0, sizeof(int32_t) * (size_t)p->num_pages, st);
+    if (e != cudaSuccess) return report_error(SFA_ERR_CUDA, std::string("cache accept: ") + cudaGetErrorString(e));
+    note_memset("cache_count", st);
+    count_kernel<<<p->num_seqs, kMove, 0, st>>>(*p);
+    note_launch("cache_count", st);
+  }
+  return sfa_cache_accept(p, stream);
 }
 
 int sfa_cache_compact(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream) {

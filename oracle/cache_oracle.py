@@ -85,8 +85,19 @@ def fork(refs, table, lens, src, dst, pools):
     return out
 
 
-def accept(pools, table, lens, accepted, drafted):
+def count(table, lens, page, num):
+    """Entries of the table that hold each page."""
+    out = [0] * num
+    for row, length in zip(table, lens):
+        for pg in row[:pages_of(length, page)]:
+            if 0 <= pg < num:
+                out[pg] += 1
+    return out
+
+
+def accept(pools, table, lens, accepted, drafted, refs=None):
     page, num = pools[0].shape[1], pools[0].shape[0]
+    refs = count(table, lens, page, num) if refs is None else refs
     keep = []
     for s, row in enumerate(accepted):
         if not 0 <= drafted[s] <= lens[s]:
@@ -98,14 +109,20 @@ def accept(pools, table, lens, accepted, drafted):
                 break
             taken.append(a)
             last = a
+        moves = []
         for i, a in enumerate(taken):
             x, y = prefix + a, prefix + i
             if max(x, y) // page >= len(table[s]):
                 continue
             px, py = table[s][x // page], table[s][y // page]
             if a != i and 0 <= px < num and 0 <= py < num:
-                for p in pools:
-                    p[py, y % page] = p[px, x % page].clone()
+                moves.append((px, x % page, py, y % page))
+        if any(refs[py] > 1 for _, _, py, _ in moves):
+            keep.append(-1)
+            continue
+        for px, x, py, y in moves:
+            for p in pools:
+                p[py, y] = p[px, x].clone()
         keep.append(prefix + len(taken))
     return keep
 
