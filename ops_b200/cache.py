@@ -116,10 +116,12 @@ def paged_cache_reserve(refcounts: torch.Tensor, block_table: torch.Tensor, cach
     go into the table and ``cache_seqlens`` grows.  Returns ``granted [n]``
     (int32): 1, or 0 where nothing was changed — a negative count, a table too
     narrow, a partly filled last page that other sequences share, or free pages
-    too few for the sequences up to this one together.  The new rows of a sequence
-    that was refused must stay out of the calls that follow (``cu_seqlens`` from
-    ``granted * rows``): its length does not include them, so they would be stored
-    over its last ones."""
+    too few for the sequences up to this one together.  The length of a sequence
+    that was refused does not include its new rows, so they would be stored over
+    its last ones: pass ``cache_seqlens * granted`` to ``qk_norm_rotary_append``
+    and ``tree_attention_paged`` (at length 0 the rows have no place and are not
+    stored, and see nothing) and ``drafted * granted`` to
+    ``paged_cache_accept``."""
     _state(refcounts, block_table, cache_seqlens, page_size)
     _ints("add", add, 1, refcounts, block_table.shape[0])
     granted = torch.empty_like(add)
