@@ -25,9 +25,9 @@
 //
 // Softmax: one thread per row.  P = exp2(S c - m) in fp32, rounded once to the
 // MMA operand's type (the row sum keeps the unrounded values).  m is not the
-// maximum but a reference: it is raised, and O rescaled in TMEM, only when a sum
-// of P exceeds 2^14, so the common pass takes no maximum.  P overwrites S's
-// columns as the PV MMA's A operand.
+// maximum but a reference, set to it (fp16: 2^8 below it, see Reference): it is raised,
+// and O rescaled in TMEM, only when a sum of P exceeds 2^14 (2^15), so the common pass
+// takes no maximum.  P overwrites S's columns as the PV MMA's A operand.
 #include "sfa_tree.cuh"
 
 #include <algorithm>

@@ -244,7 +244,7 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
             }
           }
           // P against the reference maximum so far.  The maximum of these keys is not needed for that: if
-          // their sum stays below kMost, so does every P (and an infinite or a first one does not), and
+          // their sum stays below `most`, so does every P (and an infinite or a first one does not), and
           // only otherwise is the reference raised and P done again.
           float part;
           for (bool again = false;; again = true) {
@@ -256,12 +256,12 @@ __device__ __forceinline__ void softmax(const Args& a, Shared& S, int wg, uint32
             float t0, t1;
             untwo(add2(sum0, sum1), t0, t1);
             part = t0 + t1;
-            const bool up = live && (part > kMost || mref == -INFINITY);
+            const bool up = live && (part > Reference<T>::most || mref == -INFINITY);
             if (again || !__any_sync(0xffffffffu, up)) break;
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaxf(s0[k], s1[k]));
-            top *= c2;
+            top = top * c2 - Reference<T>::below;
             float fac = 1.f;
             if (up && top > mref) {
               if (mref != -INFINITY) fac = ex2(mref - top);

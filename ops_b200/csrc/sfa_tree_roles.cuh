@@ -9,7 +9,20 @@ namespace sfa {
 namespace tree {
 
 constexpr int kRing = 8;             // key masks and scrub results: more chunks than are in flight
-constexpr float kMost = 16384.f;     // of P: far inside fp16, and sums of it far inside fp32
+
+// P is taken against a reference 2^below below the largest score seen when it was set, and the reference is
+// raised when a sum of P passes `most`: so every P is far inside the type, and sums far inside fp32.  bf16
+// has fp32's range.  In fp16, P below 2^-14 loses bits and below 2^-25 is gone while the row sum keeps it; with the
+// reference at the maximum, one key that takes all left the others of a cache of 16384 up to 16 times the
+// rounding of the rest off.  2^8 below, 64 keys as large as the largest still sum to half of `most`.
+template <typename T>
+struct Reference {
+  static constexpr float most = 16384.f, below = 0.f;
+};
+template <>
+struct Reference<__half> {
+  static constexpr float most = 32768.f, below = 8.f;
+};
 
 template <int KEYS, int THREADS, int ID>
 struct Kernel {
