@@ -302,9 +302,9 @@ int sfa_indexer_topk(const SfaIndexerParams* p, void* workspace, size_t workspac
  *     y = n with the pairs of its dims [start, start + rot) turned by
  *         position * frequencies[i] and scaled by amplitude (SFA_ROTARY_TURN)
  * rounded once to the tensor's type.  Pair i is (i, i + rot/2) of the rotated
- * part, or (2i, 2i + 1) when interleaved.  Angles are reduced exactly: the
- * position multiplies the frequency as a 64-bit fraction of a turn, so far
- * positions keep full accuracy.  dim is at most 1024, and a tensor has fewer than
+ * part, or (2i, 2i + 1) when interleaved.  Angles are reduced in whole numbers:
+ * the position multiplies the frequency as a fraction of a turn (127 bits with
+ * pos64, 64 without), so any position has the accuracy of the first ones.  dim is at most 1024, and a tensor has fewer than
  * 2^31 rows.
  *
  * Up to three tensors go through one launch (q, k and, for the append, v with

@@ -5,9 +5,9 @@
 //   dn = R^T dy,  dx = r (dn w - x r^2 mean(dn w x)),  dw = sum_rows dn x r
 //
 // The angle of a pair is position * frequency.  The frequency is held as a
-// 64-bit fraction of a turn, so the product modulo 2^64 is the exact fraction
-// of the turn (no table, no range reduction in floating point): positions of
-// any size keep the accuracy of sincospif.
+// 64-bit fraction of a turn, and what that leaves over as 63 bits more, so the
+// product modulo one turn is taken in whole numbers (no table, no range reduction
+// in floating point): positions of any size keep the accuracy of sincospif.
 //
 // Memory-bound: every row is read once and written once, in fp32 registers
 // between.  A row is spread over L lanes, each with two runs of P elements, so
@@ -36,15 +36,27 @@ template <> __device__ __forceinline__ float from_f<float>(float x) { return x; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
-// A frequency (radians per position) as a 64-bit fraction of a turn.
-__device__ __forceinline__ uint64_t turn_step(double f) {
-  double t = f * 0.15915494309189533577;
-  t -= floor(t);
-  return __double2ull_rn(t * 18446744073709551616.0);
+// A frequency (radians per position) as a fraction of a turn: units of 2^-64, and the rest in units of 2^-127.
+struct Step {
+  uint64_t units;
+  int64_t rest;
+};
+__device__ __forceinline__ Step turn_step(double f) {
+  // f / 2 pi as hi + lo; 1 / 2 pi rounded to a double, and what that leaves over
+  constexpr double k1 = 0.15915494309189535, k2 = -9.839338337591243e-18;
+  const double g = fabs(f), hi = g * k1, lo = fma(g, k2, fma(g, k1, -hi));
+  const double u = (hi - floor(hi)) * 18446744073709551616.0;               // exact, below 2^64
+  const double whole = floor(u), v = (u - whole) + lo * 18446744073709551616.0, n = rint(v);
+  Step s{__double2ull_rz(whole) + (uint64_t)__double2ll_rn(n), __double2ll_rn((v - n) * 9223372036854775808.0)};
+  if (f < 0.0) s = Step{0 - s.units, -s.rest};
+  return s;
 }
 
-__device__ __forceinline__ void turn(uint64_t step, int64_t pos, float amplitude, float& c, float& s) {
-  const int32_t hi = (int32_t)((step * (uint64_t)pos) >> 32);
+// `far`: 64-bit positions, for which the rest counts (2^31 positions of half a unit are 2^-34 of a turn).
+__device__ __forceinline__ void turn(Step step, int64_t pos, bool far, float amplitude, float& c, float& s) {
+  uint64_t units = step.units * (uint64_t)pos;
+  if (far) units += 2 * (uint64_t)__mul64hi(step.rest, pos);
+  const int32_t hi = (int32_t)(units >> 32);
   sincospif((float)hi * 4.656612873077393e-10f, &s, &c);   // hi / 2^31 half turns
   c *= amplitude;
   s *= amplitude;
@@ -286,7 +298,7 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = lane % L, sub = lane / L, pairs = p.rot >> 1;
   uint8_t* ring = smem + threadIdx.x * R;                      // run k of stage s at (s * K + k) * kWarps * 32 * R
-  uint64_t* steps = reinterpret_cast<uint64_t*>(smem + ring_bytes<T, P, NS, BWD>());
+  Step* steps = reinterpret_cast<Step*>(smem + ring_bytes<T, P, NS, BWD>());
   float2* cs = reinterpret_cast<float2*>(steps + pairs) + warp * pairs;
   int ti = 0, cta = blockIdx.x;
   while (cta >= g.ctas[ti]) cta -= g.ctas[ti++];
@@ -401,7 +413,7 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
 #pragma unroll 1
         for (int i = lane; i < pairs; i += 32) {
           float cc, ss;
-          turn(steps[i], pos, p.amplitude, cc, ss);
+          turn(steps[i], pos, p.pos64, p.amplitude, cc, ss);
           cs[i] = make_float2(cc, ss);
         }
         __syncwarp();
@@ -588,7 +600,7 @@ rotary_any_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_consta
       db = bb >= 0 ? to_f(dy[bb]) : 0.f;
       if (j < half) {
         float c, s;
-        turn(turn_step(__ldg(p.frequencies + j)), pos, p.amplitude, c, s);
+        turn(turn_step(__ldg(p.frequencies + j)), pos, p.pos64, p.amplitude, c, s);
         const float u = da * c + db * s, v = db * c - da * s;
         da = u;
         db = v;
@@ -630,7 +642,7 @@ rotary_any_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_consta
         ob = nb;
         if (j < half) {
           float c, s;
-          turn(turn_step(__ldg(p.frequencies + j)), pos, p.amplitude, c, s);
+          turn(turn_step(__ldg(p.frequencies + j)), pos, p.pos64, p.amplitude, c, s);
           oa = na * c - nb * s;
           ob = nb * c + na * s;
         }
@@ -742,7 +754,7 @@ static int total_ctas(const SfaRotaryParams& p, const Grid& g) {
 
 template <typename T, int P, int L, int NS, bool BWD, bool INTER>
 static void launch_layout(const SfaRotaryParams& p, const Grid& g, cudaStream_t st) {
-  const size_t turns = (size_t)(p.rot / 2) * (sizeof(uint64_t) + kWarps * sizeof(float2));   // at most 36 KB
+  const size_t turns = (size_t)(p.rot / 2) * (sizeof(Step) + kWarps * sizeof(float2));   // at most 40 KB
   const size_t smem = std::max(ring_bytes<T, P, NS, BWD>() + turns, BWD ? kWarps * sizeof(float) * p.dim : (size_t)0);
   if (smem > 48 * 1024)
     cudaFuncSetAttribute(rotary_kernel<T, P, L, NS, BWD, INTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
