@@ -257,6 +257,42 @@ def _check_pool(name: str, c: torch.Tensor, like: torch.Tensor):
     return shape, stride
 
 
+def _rows_meet(rows: int, heads: int, d: int, st: int, sh: int) -> bool:
+    """Whether different rows or heads of a pool share elements."""
+    if rows > 1 and st < d or heads > 1 and sh < d:
+        return True
+    if rows < 2 or heads < 2 or st >= (heads - 1) * sh + d or sh >= (rows - 1) * st + d:
+        return False                       # heads inside a row, or rows inside a head
+    for j in range(1, heads):              # a head j further on, and the rows around it
+        i, r = divmod(j * sh, st)
+        if i < rows and r < d or i + 1 < rows and st - r < d:
+            return True
+    return False
+
+
+def _pools_meet(rows: int, heads: int, k, v) -> bool:
+    """Whether two pools share elements; k and v: (first element, row stride, head
+    stride, head size), all in elements."""
+    (k0, kst, ksh, dk), (v0, vst, vsh, dv) = k, v
+    if rows < 1 or v0 >= k0 + (rows - 1) * kst + (heads - 1) * ksh + dk or k0 >= v0 + (rows - 1) * vst + (heads - 1) * vsh + dv:
+        return False
+    if rows > 1 and kst != vst:
+        return True                        # one inside the other with rows of its own: not a layout of two pools
+    st, at = kst if rows > 1 else max(kst, vst, 1), v0 - k0
+    r = at % st
+    if (heads - 1) * ksh + dk <= r and r + (heads - 1) * vsh + dv <= st:
+        return False                       # [rows, 2, heads, D]
+    if ksh == vsh and ksh > 0 and st % ksh == 0 and dk <= r % ksh and r % ksh + dv <= ksh:
+        return False                       # [rows, heads, 2, D]
+    for a in range(heads):
+        for b in range(heads):
+            x = at + b * vsh - a * ksh     # head b of v behind head a of k; rows i apart move it by i * st
+            for i in range(-((x + dv - 1) // st), (dk - 1 - x) // st + 1):
+                if -rows < i < rows:
+                    return True
+    return False
+
+
 def _check_table(block_table: torch.Tensor, cache_seqlens: torch.Tensor, like: torch.Tensor):
     """(sequences, pages of a row of the table)."""
     for name, t, d in (("block_table", block_table, 2), ("cache_seqlens", cache_seqlens, 1)):
@@ -302,7 +338,7 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
         (n, m, h, d), (_, st, sh, _) = pools[-1]
         if c.dtype != dtype or h != rows[1] or d != rows[2]:
             raise ValueError(f"{name} must have the type, heads and head size of the rows stored into it")
-        if n * m > 1 and st < d or h > 1 and sh < d:
+        if _rows_meet(n * m, h, d, st, sh):
             raise ValueError(f"{name}: rows and heads must not overlap, they are stored into")
     (num_pages, page, _, _), kst = pools[0]
     (v_pages, v_page, _, _), vst = pools[1]
@@ -310,6 +346,10 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
         raise ValueError("k_cache and v_cache must have the same pages")
     if k_cache.data_ptr() == v_cache.data_ptr() != 0:
         raise ValueError("k_cache and v_cache must not be the same memory")
+    size = dtype.itemsize
+    if _pools_meet(num_pages * page, ks[1], (k_cache.data_ptr() // size, kst[1], kst[2], ks[2]),
+                   (v_cache.data_ptr() // size, vst[1], vst[2], vs[2])):
+        raise ValueError("k_cache and v_cache must not share elements")
     n, width = _check_table(block_table, cache_seqlens, q)
     if cu_seqlens is None:
         if qs[0] != n:
