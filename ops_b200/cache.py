@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from operator import sub
 from typing import Optional, Sequence
 
 import torch
@@ -32,6 +33,32 @@ def _ints(name: str, t: torch.Tensor, dim: int, like: torch.Tensor, size: Option
         raise ValueError(f"{name} must have {size} entries, got {t.shape[0]}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dim (it is used in place)")
+
+
+def _pools_meet(values, num_pages: int) -> bool:
+    """Whether pools share memory; values: (address, page stride, page bytes) of each, one after another."""
+    bases, strides, sizes = values[::3], values[1::3], values[2::3]
+    stride, size = strides[0], sizes[0]
+    if strides.count(stride) == len(strides) and sizes.count(size) == len(sizes):
+        at = sorted(bases)                             # pools alike, one behind the other or side by side in a page
+        gap = min(map(sub, at[1:], at), default=stride)
+        if gap >= (num_pages - 1) * stride + size or gap >= size and at[-1] + size - at[0] <= stride:
+            return False
+    spans = sorted(p for p in zip(bases, strides, sizes) if p[2] and num_pages > 0)
+    for i, (base, stride, size) in enumerate(spans):
+        last = base + (num_pages - 1) * stride + size
+        for base2, stride2, size2 in spans[i + 1:]:
+            if base2 >= last:
+                break
+            # pages of one stride lie in one another's gaps, or they meet
+            r = base2 - base
+            if num_pages > 1:
+                if stride2 != stride:
+                    return True
+                r %= stride
+            if r < size or num_pages > 1 and r + size2 > stride:
+                return True
+    return False
 
 
 def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Optional[int]):
@@ -66,6 +93,8 @@ def _pool_array(pools: Sequence[torch.Tensor], like: torch.Tensor, num_pages: Op
     held = [ptr for ptr in values[::3] if ptr]
     if len(set(held)) < len(held):
         raise ValueError("a pool is named twice")
+    if _pools_meet(values, lead[0]):
+        raise ValueError("pools must not share memory")
     arr = (SfaCachePool * len(pools)).from_buffer_copy(struct.pack("@" + "Pqq" * len(pools), *values))
     return arr, lead[0], lead[1]
 
