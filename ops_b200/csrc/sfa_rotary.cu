@@ -802,7 +802,7 @@ static int check(const SfaRotaryParams* p, bool bwd) {
   if (p->num_tensors < 1 || p->num_tensors > 3) return bad("num_tensors must be 1, 2 or 3");
   if (p->batch < 0 || p->len < 0) return bad("batch and len must be >= 0");
   if (p->dim < 1 || p->dim > kMaxDim) return bad("dim must be in [1, " + std::to_string(kMaxDim) + "]");
-  if (p->rot < 0 || p->rot % 2 || p->start < 0 || p->start + p->rot > p->dim)
+  if (p->rot < 0 || p->rot % 2 || p->rot > p->dim || p->start < 0 || p->start > p->dim - p->rot)
     return bad("rot must be even and [start, start + rot) within the head");
   if (p->dtype != SFA_DTYPE_BF16 && p->dtype != SFA_DTYPE_F16 && p->dtype != SFA_DTYPE_F32) return bad("unknown dtype");
   const bool empty = p->batch == 0 || p->len == 0;
