@@ -442,8 +442,10 @@ static int check(const SfaCacheParams* p, const char* what, bool refs, bool tabl
   // which of the fields a call reads: reference counts, table and lengths, pools, the second argument
   // array; whether the arrays go by sequence (rows) or by count
   if (!p) return bad(what, "params is NULL");
-  if (p->num_pools < 0 || p->num_seqs < 0 || p->num_pages < 0 || p->table_width < 0 || p->count < 0 || p->count >= kNone)
-    return bad(what, "sizes must be >= 0");
+  // strip() adds the threads to a size, and kNone is no index
+  if (p->num_pools < 0 || p->num_seqs < 0 || p->num_pages < 0 || p->table_width < 0 || p->count < 0 || p->num_seqs >= kNone ||
+      p->num_pages >= kNone || p->count >= kNone)
+    return bad(what, "sizes must be >= 0 and below " + std::to_string(kNone));
   if (p->page_size < 1) return bad(what, "page_size must be positive");
   if (refs && p->num_pages > 0 && !p->refcounts) return bad(what, "refcounts must be non-NULL");
   if (table && p->num_seqs > 0 && (!p->cache_seqlens || (p->table_width > 0 && !p->block_table)))

@@ -24,3 +24,20 @@ def test_rotated_part_outside_the_head(bad):
     for call in (lambda: lib.sfa_rotary_fwd(ctypes.byref(P), None), lambda: lib.sfa_rotary_bwd(ctypes.byref(P), None, 0, None)):
         assert call() == _lib.SFA_ERR_INVALID_ARGUMENT
         assert "rot" in lib.sfa_last_error_string().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(num_pages=MOST), dict(num_seqs=MOST), dict(num_pages=MOST - 1000), dict(num_seqs=MOST - 1000)])
+@pytest.mark.parametrize("name", ["reserve", "trim", "fork", "accept", "accept_table", "compact", "copy"])
+def test_state_whose_strips_would_wrap(name, bad):
+    # the bookkeeping CTA cuts pages and sequences into strips of whole numbers of 32 bits
+    lib = _lib.load()
+    arr = (_lib.SfaCachePool * 1)()
+    arr[0].base, arr[0].page_stride, arr[0].page_bytes = FAKE, 64, 64
+    P = _lib.SfaCacheParams(refcounts=FAKE, block_table=FAKE, cache_seqlens=FAKE, a=FAKE, b=FAKE, out=FAKE, pools=arr,
+                            bt_stride=4, a_stride=2, num_pools=1, num_seqs=2, num_pages=8, page_size=16, table_width=4, count=2)
+    for n, v in bad.items():
+        setattr(P, n, v)
+    f = getattr(lib, "sfa_cache_" + name)
+    code = f(ctypes.byref(P), None) if name in ("trim", "accept", "accept_table") else f(ctypes.byref(P), None, 0, None)
+    assert code == _lib.SFA_ERR_INVALID_ARGUMENT
+    assert "sizes" in lib.sfa_last_error_string().decode()
