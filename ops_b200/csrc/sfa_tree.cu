@@ -213,6 +213,9 @@ static int check(const SfaTreeParams* p) {
   if (p->parents && p->max_q > kMaxNodes) return bad("a tree has at most " + std::to_string(kMaxNodes) + " drafted rows a sequence");
   if ((int64_t)p->num_pages * p->page_size >= INT32_MAX)
     return report_error(SFA_ERR_UNSUPPORTED, "tree attention: a pool has fewer than 2^31 rows");
+  // units first: their product with the tiles or chunks of one stays inside 64 bits, and a strip of
+  // sequences inside 32
+  if ((int64_t)p->num_seqs * p->h_kv >= (1 << 30)) return report_error(SFA_ERR_UNSUPPORTED, "tree attention: too many sequences and heads");
   const int64_t chunks = ((int64_t)p->table_width * p->page_size + 63) / 64;
   if (chunks * p->num_seqs * p->h_kv >= INT32_MAX || (int64_t)p->table_width * p->page_size >= INT32_MAX)
     return report_error(SFA_ERR_UNSUPPORTED, "tree attention: table too large");

@@ -41,3 +41,18 @@ def test_state_whose_strips_would_wrap(name, bad):
     code = f(ctypes.byref(P), None) if name in ("trim", "accept", "accept_table") else f(ctypes.byref(P), None, 0, None)
     assert code == _lib.SFA_ERR_INVALID_ARGUMENT
     assert "sizes" in lib.sfa_last_error_string().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(num_seqs=MOST, h_q=MOST, h_kv=MOST), dict(num_seqs=2 ** 30, h_q=2 ** 30, h_kv=2 ** 30, table_width=2 ** 20),
+                                 dict(num_seqs=2 ** 31 - 100, h_q=1, h_kv=1, table_width=1), dict(num_seqs=2 ** 16, h_q=2 ** 15, h_kv=2 ** 15)])
+def test_tree_units_that_would_wrap(bad):
+    # sequences times heads times tiles (or chunks) may pass 64 bits
+    lib = _lib.load()
+    P = _lib.SfaTreeParams(q=FAKE, k=FAKE, v=FAKE, block_table=FAKE, cache_seqlens=FAKE, cu_seqlens=FAKE, o=FAKE, lse=FAKE,
+                           q_st=512, q_sh=64, k_st=128, k_sh=64, v_st=128, v_sh=64, o_st=512, o_sh=64, l_st=8, l_sh=1,
+                           bt_stride=4, num_seqs=2, total_q=6, max_q=4, max_k=64, h_q=8, h_kv=2, d_qk=64, d_v=64, num_pages=8,
+                           page_size=16, table_width=0, scale=0.125)
+    for n, v in bad.items():
+        setattr(P, n, v)
+    assert lib.sfa_tree_attention(ctypes.byref(P), None, 0, None) == _lib.SFA_ERR_UNSUPPORTED
+    assert lib.sfa_tree_workspace_bytes(ctypes.byref(P)) == 0
