@@ -582,8 +582,8 @@ int sfa_cache_accept_table(const SfaCacheParams* p, void* stream) {
 
 int sfa_cache_compact(const SfaCacheParams* p, void* workspace, size_t workspace_bytes, void* stream) {
   SfaCacheParams q0 = p ? *p : SfaCacheParams{};
-  q0.cache_seqlens = q0.cache_seqlens ? q0.cache_seqlens : q0.refcounts;   // no lengths, no argument arrays
-  q0.a = q0.a ? q0.a : q0.refcounts;
+  q0.cache_seqlens = q0.cache_seqlens ? q0.cache_seqlens : q0.out;   // no lengths, no argument arrays
+  q0.a = q0.a ? q0.a : q0.out;
   int rc = check(p ? &q0 : nullptr, "compact", true, true, true, false, true);
   if (rc) return rc;
   if (!p->out) return bad("compact", "the output must be non-NULL");
