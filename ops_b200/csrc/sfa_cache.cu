@@ -11,8 +11,10 @@
 // the bookkeeping left in the workspace.  Measured: 2.35 GB read and written to
 // move some 1100 pages of 128 KB in each of 8 pools in 394 us (0.91 of the measured copy
 // rate); a beam step of 64 sequences (trim, fork, its 32 pages in 16 pools, reserve) in
-// 35 us, 20.5 of them the pages' floor; acceptance and trim of 128 trees in 32 pools in
-// 20 us, a chain of dependent reads (lengths, path, table, rows) around 10 us of rows.
+// 37 us, 20.5 of them the pages' floor; acceptance and trim of 128 trees in 32 pools in
+// 21 us, a chain of dependent reads (lengths, path, table, counts, rows) around 10 us of
+// rows, and in 24 us where acceptance counts the table's entries itself (both with 6 us
+// that restore the state between calls).
 #include "sfa_common.cuh"
 #include "sfa_internal.h"
 
@@ -65,7 +67,9 @@ static size_t carve(const SfaCacheParams& p, char* ws, Work* w) {
 
 __device__ __forceinline__ int pages_of(int rows, int page_size) { return rows > 0 ? (rows - 1) / page_size + 1 : 0; }
 
-// Exclusive sum of v over the CTA's threads in order; *total: the sum.  Starts and ends with a barrier.
+// Exclusive sum of v over the CTA's threads in order; *total: the sum.  A barrier before part[] is written and
+// one after it, none once it has been read: what a thread wrote before or writes after the call is not yet
+// there for the others.
 template <typename N>
 __device__ __forceinline__ N block_scan(N v, N* total) {
   __shared__ N part[kPlan / 32];
@@ -554,7 +558,7 @@ int sfa_cache_accept(const SfaCacheParams* p, void* stream) {
   by_pools(*p, true, [&](const SfaCacheParams& q, const Pools& t, int first) {
     // threads a pool: as many as the widest row has units; CTAs: one wave of eight per SM, each with
     // several pools (with a CTA for each sequence and pool, acceptance and trim of 128 sequences in 32 pools
-    // took 31 us instead of 20)
+    // took 11 us more)
     int lanes = 32;
     for (int k = 0; k < q.num_pools; ++k)
       while (lanes < kMove && t.t[k].page_bytes / q.page_size > 16 * (int64_t)lanes) lanes *= 2;

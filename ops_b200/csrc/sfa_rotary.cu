@@ -289,6 +289,9 @@ struct Steps {
 // heads of 128, against 507 us here (436 us would be the five passes over q and k at copy rate; instruction
 // issue is 74 % busy in the forward, 62 % in the backward).  Forward: 3 CTAs per SM (20 us more with 2; the
 // backward's registers allow 2).
+// Two units a lane (above 512 dims of 16 bits, 256 of fp32) do not fit: the backward spills 510 to 550 bytes a
+// thread, the forward 44 to 72, and 28 of the 64 lane slots idle at 576 dims.  8192 tokens of 16 + 1 heads of 576:
+// forward 119 us for 49 of bytes, the step with gradients 682 for 123; of 512: 76 for 44, 213 for 109.
 // Dynamic shared memory: the ring, the turn steps of the rot / 2 pairs, their (cos, sin) for each warp's token.
 template <typename T, int P, int L, int NS, bool BWD, bool INTER>
 __global__ void __launch_bounds__(kWarps * 32, BWD || NS > 1 ? 2 : 3)
@@ -550,7 +553,9 @@ rotary_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__
 }
 
 // Any head size, offset, stride and alignment: one warp per row, one element at
-// a time, a pair in one lane.
+// a time, a pair in one lane, the angle of every pair anew for every head.  Bound by
+// that: 16384 tokens of 16 + 4 heads of 80 with 20 dims turned take 205 us forward and
+// 562 with gradients, with 32 turned (the kernel above) 43 and 110.
 template <typename T, bool BWD>
 __global__ void __launch_bounds__(kWarps * 32)
 rotary_any_kernel(const __grid_constant__ SfaRotaryParams p, const __grid_constant__ Grid g) {
@@ -686,7 +691,8 @@ struct Shape {
   int p, lanes, units;
 };
 
-// The widest runs that sizes and alignment allow: every run of P elements starts at a multiple of P.
+// The widest runs that sizes and alignment allow: every run of P elements starts at a multiple of P, so head
+// size, rotated part and its start are multiples of 8 at least, in every tensor of the call.
 static Shape shape_of(const SfaRotaryParams& p, bool bwd) {
   const int size = p.dtype == SFA_DTYPE_F32 ? 4 : 2;
   auto fits = [&](int n) {

@@ -12,11 +12,17 @@
 // decode step is bound by those reads, a large tree by the MMAs and the softmax.
 //
 // Split: the (sequence, kv head, chunk of keys) space of all sequences is one line
-// that gridDim.x CTAs cut into equal ranges, whatever the lengths; a CTA walks the
-// units (sequence, kv head) its range touches.  A unit that lies in one range is
+// that gridDim.x CTAs cut into equal ranges, whatever the lengths of the caches; a CTA
+// walks the units (sequence, kv head) its range touches.  A unit that lies in one range is
 // finished there; pieces of the others go to a workspace as (m, l, O) and
 // tree_combine_kernel joins them in range order.  The gridDim.y row tiles of a
-// unit walk the same range at the same time and share its reads in L2.
+// unit walk the same range at the same time and share its reads in L2.  The line does
+// not count rows: gridDim.y comes from the longest sequence of drafted rows (max_q),
+// gridDim.x is what is left of the SMs, and of a sequence with fewer rows only the CTAs
+// of its own tiles work.  Rows of very different numbers therefore belong in calls of
+// their own: 63 single tokens over 4096 to 32768 keys take 846 us and one chunk of 2048
+// rows 706, both in one call 47.7 ms (64 tile pairs leave two ranges); 15 single tokens
+// take 239 us and a chain of 64 rows 52, together 666.
 //
 // Keys come through the block table with TMA boxes of as many rows as divide both
 // a page and a chunk, 128B-swizzled 64-dim slabs; a box without a page (a table

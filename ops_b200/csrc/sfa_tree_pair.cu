@@ -13,7 +13,7 @@
 // A CTA goes by piece: it falls back to `keys` where its second tile is empty.
 //
 // Measured: one token for each of 16 sequences of 4096 to 32768 keys, 64 heads on
-// 8, 178 us at 5.2 TB/s (0.79 of the measured copy rate); 64-node trees on 8
+// 8, 179 us at 5.1 TB/s (0.79 of the measured copy rate); 64-node trees on 8
 // sequences 244 us, 790 TFLOP/s (0.48 of the measured peak).  There a period of
 // 4600 clocks covers 128 keys for both tiles: 2300 from S to P (1024 of them the
 // exponentials' floor) and 2300 from P to the next S (1024 of them MMAs).  Not

@@ -4,8 +4,8 @@
 // O takes up to 256 columns of TMEM, two S tiles of 64 keys another 128: one softmax warpgroup, and the
 // S of the next chunk is computed while it works on this one's.  64 keys a chunk: Q of 256 dims takes
 // 64 KB of shared memory, a stage of the K or V ring 32 KB.  Measured at 256 dims: one
-// cache of 131072 keys, 2 kv heads of 8 query heads, 16 drafted rows, 77 us (3.5 TB/s,
-// 17 of them the join of 148 pieces); 64-node trees on 8 sequences 135 us (710 TFLOP/s).
+// cache of 131072 keys, 2 kv heads of 8 query heads, 16 drafted rows, 78 us (3.5 TB/s,
+// 17 of them the join of 148 pieces); 64-node trees on 8 sequences 132 us (732 TFLOP/s).
 //
 // Warps: 0 K, Q and key masks; 1 V; 2 MMA issue; 3 clears value rows that must not enter a product (see
 // scrub); 4-7 softmax.  Every wait is bounded (~2 s); on expiry the kernel records (7 << 16) | site in

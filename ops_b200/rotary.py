@@ -38,7 +38,11 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     * ``"yarn"``: pairs that turn more than ``beta_fast`` times in
       ``original_length`` positions stay, those that turn less than
       ``beta_slow`` times are divided by ``factor``, those between are blended
-      linearly in their number of turns; the amplitude is ``0.1 ln(factor) + 1``.
+      linearly in their number of turns, as the method was published; the
+      amplitude is ``0.1 ln(factor) + 1``.  Checkpoints made with the public
+      implementation blend linearly in the pair's index between the two pairs
+      that turn ``beta_fast`` and ``beta_slow`` times instead, which gives the
+      pairs between other frequencies: pass theirs as ``frequencies``.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be a positive even number")
@@ -219,7 +223,9 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, frequencies: torc
     start + 2 * len(frequencies))`` of every head are turned pair by pair by
     ``position * frequency`` and scaled by ``amplitude``, the others are copied.
     Pairs are ``(i, i + rotary_dim / 2)``, or neighbours when ``interleaved``.
-    ``positions`` (int32 or int64) broadcast to the tokens.  Differentiable in x."""
+    ``positions`` (int32 or int64) broadcast to the tokens.  Differentiable in x.
+    Head sizes, rotated parts and starts that are not multiples of 8, and rows
+    that are not aligned to 8 bytes (fp32: 16), take a kernel about five times slower."""
     _check("x", x)
     if frequencies is None or positions is None:
         raise ValueError("rotary_embedding needs positions and frequencies")

@@ -54,7 +54,10 @@ def tree_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``lse = -inf`` (or its sink); so do rows outside all sequences.
 
     ``max_seqlen_q`` must cover the longest sequence of drafted rows; left unset
-    with ``cu_seqlens`` it is read back with a host sync.  ``max_seqlen_k`` is an
+    with ``cu_seqlens`` it is read back with a host sync.  It also decides how the
+    GPU is shared out: where it is many times what most sequences have (a chunk of
+    a prompt among single tokens), those run on a part of the GPU, so give such
+    sequences calls of their own.  ``max_seqlen_k`` is an
     estimate of the longest cache that sizes the split of the work (default:
     what the table covers)."""
     if q.dtype not in _DTYPE:
