@@ -122,7 +122,7 @@ def test_random_histories_with_forks_before_acceptance(counts, shapes, n, width,
 @pytest.mark.parametrize("shapes", SHAPES, ids=["vectors", "bytes", "large"])
 @pytest.mark.parametrize("n,width,pages,seed", [(9, 6, 60, 1), (40, 5, 250, 2), (4, 12, 50, 3)])
 def test_drafts_forked_and_accepted(counts, shapes, n, width, pages, seed):
-    # every round: room for drafts in a third of the rows, those forked into the empty ones, acceptance on all
+    # every step: room for drafts in a third of the rows, those forked into the empty ones, acceptance on all
     r, c = random.Random(seed), cache(counts, n, width, pages, shapes, seed)
     refused = moved = 0
     for step in range(8):
